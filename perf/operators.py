@@ -280,8 +280,8 @@ def work(case):
     if op in ("norm", "norm_train"):
         io = rows * (k * (3 * b + 1 + 2) + blocks) + 4 * k          # x, residual, sum; codes, values, scales
         fl = 8 * rows * k
-        if op == "norm_train":                                       # dy, dh, dx; the sum is an input again
-            io += rows * k * 4 * b + 8 * k
+        if op == "norm_train":                                       # dy, dh, dx, dgain
+            io += rows * k * 3 * b + 4 * k
             fl += 12 * rows * k
         return {"bytes": io, "flops": fl}
     if op == "quantise":

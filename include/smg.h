@@ -36,7 +36,7 @@ enum { SMG_MEM_DEVICE = 0, SMG_MEM_HOST = 1 };
 #define SMG_WALL_SEGS_MAX 1024
 /* the wall state vector (sm_snap_wall_state, scenemap include/scenemap.h:96-99) */
 #define SMG_WALL_STATE_LEN 56
-enum { SMG_EMB_F32 = 0, SMG_EMB_BF16 = 1 };
+enum { SMG_EMB_F32 = 0, SMG_EMB_BF16 = 1, SMG_EMB_F16 = 2 };   /* F16: the embedding heads only */
 
 /* Parameters.  Field names and defaults mirror the reference structs:
  * ObjParams (scenemap include/scenemap/objmap.hpp:50-129), ApParams (objprob.hpp:56-142),
@@ -547,6 +547,77 @@ int smg_assoc_error(smg_assoc* a);
  * landed, 5 all MMAs done, 6 epilogue done, 7 exit, 8-11 epilogue steps); out16 (or NULL)
  * receives the last record. */
 int smg_assoc_stamps(smg_assoc* a, int enable, int64_t* out16);
+
+/* ---- embedding heads: ragged products by map, residual norm, microscaled rows ----
+ * A map's head turns image embeddings into that map's own (h = x + W_g x, normalised), and the
+ * normalised rows are compared with the map's memory bank.  No counterpart in the reference,
+ * which uses the image model's embeddings as they are.
+ *
+ * Common to these calls: all pointers are device memory of the current device unless said
+ * otherwise, and the call is asynchronous on `stream`, allocates nothing and keeps nothing.
+ * `type` is SMG_EMB_F32 / SMG_EMB_BF16 / SMG_EMB_F16.  Leading dimensions (ld*) count elements
+ * from one row to the next.  The rows of all groups (maps) are packed: group g has the rows
+ * off[g] .. off[g+1] - 1 (off: n_groups + 1 device entries, off[0] = 0, off[n_groups] = rows, never
+ * decreasing; a group may be empty).  off = NULL means one group of all rows (n_groups = 1).
+ * err (may be NULL) is a device word that gets SMG_PROD_TIMEOUT or'ed in when a wait inside the
+ * kernel ran out and SMG_PROD_OFFSETS when off breaks these rules (a group with bad offsets is
+ * taken as empty; nothing outside the arrays is read or written).  n_groups <= 1024. */
+#define SMG_PROD_MAX_GROUPS 1024
+enum { SMG_PROD_TIMEOUT = 1, SMG_PROD_OFFSETS = 2 };
+/* y[r][j] = sum_i x[r][i] w[g][j][i] for the rows r of group g: x rows x k, w n_groups x n x k (row j
+ * of group g at w + g * w_stride + j * ldw), y rows x n.  x and w are bf16 or f16 (`type`), y is
+ * y_type.  Sums are kept in 32 bits and rounded once.  x and w: 16-byte aligned base and rows (ld
+ * and w_stride multiples of 8); k and n are free. */
+int smg_group_product(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t w_stride, const int32_t* off, int n_groups,
+                      int rows, int n, int k, int type, void* y, int64_t ldy, int y_type, int32_t* err, void* stream);
+/* Gradient for x: dx[r][i] = sum_j dy[r][j] w[g][j][i].  dy rows x n and w aligned as above. */
+int smg_group_product_dx(const void* dy, int64_t lddy, const void* w, int64_t ldw, int64_t w_stride, const int32_t* off,
+                         int n_groups, int rows, int n, int k, int type, void* dx, int64_t lddx, int dx_type, int32_t* err,
+                         void* stream);
+/* Gradient for w: dw[g][j][i] = sum over the rows r of group g of dy[r][j] x[r][i]; zeros for an
+ * empty group.  dw at dw + g * dw_stride + j * lddw.  The sum's order is fixed: equal inputs give
+ * equal bits. */
+int smg_group_product_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int32_t* off, int n_groups, int rows,
+                         int n, int k, int type, void* dw, int64_t lddw, int64_t dw_stride, int dw_type, int32_t* err,
+                         void* stream);
+
+/* Microscaled rows (the OCP microscaling formats MXFP4 and MXFP8 with e4m3): every 32 values of a
+ * row share a power of two 2^e, e = floor(log2(largest magnitude)) - emax, clamped to -127..127 (emax 2
+ * for bits = 4, e2m1; 8 for bits = 8, e4m3; an all-zero block gets -127); each value x is kept as
+ * x / 2^e rounded to the nearest (ties to even), the format's largest magnitude (6, 448) where it
+ * is above.  A block that holds an infinity or NaN gets the scale NaN.
+ * codes: rows of ceil(k/32)*32*bits/8 bytes (4 bits: element 2i in the low half of byte i), zeros
+ * past k.  scales: rows of ceil(k/128)*4 bytes, e + 127 (255 = NaN), zeros past the last block.
+ * Both 16-byte aligned.  values (may be NULL): the values that the codes stand for, bf16 (exact but
+ * for magnitudes below 2^-126), rows x k packed.  codes and scales may be NULL together when
+ * values is given. */
+int smg_mx_quantise(const void* x, int64_t ldx, int rows, int k, int type, int bits, uint8_t* codes, uint8_t* scales,
+                    uint16_t* values, void* stream);
+/* The values that microscaled rows stand for, as out_type (leading dimension ld). */
+int smg_mx_values(const uint8_t* codes, const uint8_t* scales, int rows, int k, int bits, void* out, int64_t ld, int out_type,
+                  void* stream);
+/* y[r][j] = sum_i a[r][i] b[g][j][i] of microscaled a (rows x k) and b (n_groups x n x k, packed), both
+ * of `bits`: the exact products of the values they stand for, summed in 32 bits. */
+int smg_mx_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales,
+                   const int32_t* off, int n_groups, int rows, int n, int k, int bits, void* y, int64_t ldy, int y_type,
+                   int32_t* err, void* stream);
+
+/* h = x + r (r may be NULL: h = x); y = h * rstd * gain with rstd = 1 / sqrt(mean(h^2) + eps), in 32
+ * bits from the unrounded sum.  x, r, h rows x dim of `type`; gain dim floats.  Outputs, each may be
+ * NULL: h, rstd (rows floats), codes and scales of y as above (bits 4 or 8), values of those codes
+ * (bf16, packed).  dim <= 16384. */
+int smg_norm_add(const void* x, int64_t ldx, const void* r, int64_t ldr, const float* gain, int rows, int dim, int type, float eps,
+                 void* h, int64_t ldh, float* rstd, int bits, uint8_t* codes, uint8_t* scales, uint16_t* values, void* stream);
+/* Its gradients, the rounding to codes taken as the identity: for dy (rows x dim, the gradient for y)
+ * and dh (or NULL: the gradient that reaches h past the norm), with n = h * rstd and u = dy * gain,
+ * dx = rstd * (u - n * mean(u * n)) + dh, which is the gradient for x and for r alike, and
+ * dgain[i] = sum over the rows of dy * n (dim floats, zeros when rows = 0; fixed order).  h is taken from x + r
+ * again (its rounded form would put its rounding into dgain).  work: smg_norm_add_bwd_work(dim)
+ * bytes of device memory, 16-byte aligned, no initial value. */
+int64_t smg_norm_add_bwd_work(int dim);
+int smg_norm_add_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* r, int64_t ldr, const float* rstd,
+                     const float* gain, const void* dh, int64_t lddh, int rows, int dim, int type, void* dx, int64_t lddx,
+                     float* dgain, void* work, void* stream);
 
 /* Batched plane fit: replaces scenemap::apPlaneFit (objprob.hpp:204, objprob.cpp:130-209), one
  * call per point set there.  Set s is the float (x, y, z) points xyz[3*off[s] .. 3*off[s+1]),

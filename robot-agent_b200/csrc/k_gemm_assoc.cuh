@@ -25,6 +25,7 @@
 #pragma once
 #include <cuda.h>
 #include "dev_util.cuh"
+#include "tc_util.cuh"
 
 #define AG_BM 128
 #define AG_BN 256
@@ -36,7 +37,6 @@
 #define AG_B_BYTES (AG_BN * AG_BK * 2)
 #define AG_TMEM_COLS 256
 #define AG_SMEM (AG_STAGES * (AG_A_BYTES + AG_B_BYTES) + 1024 + 256 + AG_BN * 8 * 4 + AG_GROUPS * AG_BM * 3 * 4)
-#define AG_WAIT_NS 200000000ull   // 0.2 s per wait
 
 // instruction descriptor, kind::f16: D f32 (bits 4-5 = 1), A bf16 (bits 7-9 = 1), B bf16
 // (bits 10-12 = 1), both K-major, N >> 3 at bits 17-22, M >> 4 at bits 24-28
@@ -61,98 +61,12 @@ struct AssocArgs {
   unsigned long long* stamps;   // optional: %globaltimer at 16 points of CTA (0, 0) (instrumentation)
 };
 
-DEV uint32_t ag_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-DEV uint64_t ag_now() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-DEV void ag_mbar_init(uint64_t* b, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(ag_smem(b)), "r"(count) : "memory");
-}
-
-DEV void ag_expect_tx(uint64_t* b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(ag_smem(b)), "r"(bytes) : "memory");
-}
-
-DEV bool ag_try_wait(uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(ag_smem(b)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// bounded wait on phase `parity`; false after AG_WAIT_NS
-DEV bool ag_wait(uint64_t* b, uint32_t parity) {
-  const uint64_t t0 = ag_now();
-  for (uint32_t i = 0;; ++i) {
-    if (ag_try_wait(b, parity)) return true;
-    if ((i & 255u) == 255u && ag_now() - t0 > AG_WAIT_NS) return false;
-  }
-}
-
-DEV void ag_tma_2d(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          ag_smem(dst)),
-      "l"((uint64_t)map), "r"(ag_smem(bar)), "r"(x), "r"(y)
-      : "memory");
-}
-
-// shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row atoms 1024 bytes apart
-DEV uint64_t ag_desc(const void* tile) {
-  const uint32_t a = ag_smem(tile);
-  uint64_t d = (uint64_t)((a >> 4) & 0x3fffu);
-  d |= (uint64_t)1 << 16;             // leading byte offset (unused for swizzled K-major)
-  d |= (uint64_t)(1024 >> 4) << 32;   // stride byte offset
-  d |= (uint64_t)1 << 46;             // descriptor version for tcgen05
-  d |= (uint64_t)2 << 61;             // SWIZZLE_128B
-  return d;
-}
-
 DEV void ag_mma(uint32_t tmem, uint64_t da, uint64_t db, uint32_t accum) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem),
       "l"(da), "l"(db), "r"(AG_IDESC), "r"(accum));
-}
-
-DEV void ag_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(ag_smem(bar)) : "memory");
-}
-
-DEV void ag_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-DEV void ag_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-DEV void ag_tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-DEV void ag_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // 3D AABB IoU > tmin, float, fixed operation order (the restatement uses the same)

@@ -49,6 +49,15 @@ static int fail(int code, const char* msg) {
   g_err = msg;
   return code;
 }
+// The error text of calls that live in other files of the library (prod.cu).
+__attribute__((visibility("hidden"))) int smg_set_error(int code, const char* msg) {
+  try {
+    g_err = msg;
+  } catch (...) {   // no memory for the text: the code still goes out, no exception does
+    g_err.clear();
+  }
+  return code;
+}
 #define CK(x)                                                     \
   do {                                                            \
     cudaError_t e_ = (x);                                         \

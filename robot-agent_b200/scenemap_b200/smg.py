@@ -134,7 +134,8 @@ EXPORTED = ["smg_params_set_cloud", "smg_params_size", "smg_params_default", "sm
            "smg_assoc_match", "smg_assoc_error", "smg_assoc_stamps", "smg_label_loglik", "smg_name", "smg_get_reencode",
            "smg_get_object_cloud_rgb", "smg_get_views", "smg_get_assoc_all_async", "smg_wait_read",
            "smg_set_text_model", "smg_get_object_name", "smg_set_walls", "smg_get_wall_segments", "smg_wall_state",
-           "smg_snapshot", "smg_ply_header"]
+           "smg_snapshot", "smg_ply_header", "smg_group_product", "smg_group_product_dx", "smg_group_product_dw",
+           "smg_mx_quantise", "smg_mx_values", "smg_mx_product", "smg_norm_add", "smg_norm_add_bwd", "smg_norm_add_bwd_work"]
 
 NUM_KERNELS = 18
 

@@ -1,109 +1,517 @@
-// Ragged products by group: y = x w_g^T, dx = dy w_g, dw_g = dy_g^T x_g, and the same first form of
-// microscaled rows.  One thread per output value.
+// Ragged products by group on the tcgen05 tensor cores: y = x w_g^T, dx = dy w_g, dw_g = dy_g^T x_g in
+// 16 bits, and y = a b_g^T of microscaled rows (e2m1 or e4m3 with a power of two for 32 values).
+//
+// All of them are D[128][BN] += P Q^T over blocks of the reduction axis, with a 128-row operand P
+// and a BN-row operand Q in a ring of shared-memory stages and the sums in tensor memory, 32 bits
+// each, two accumulators in turn.  The forms differ in what P and Q are and how they lie:
+//
+//   FORM    P (128 rows)           Q (BN rows)              reduction   D
+//   Y       rows of x              rows of w_g              k           rows x n
+//   Y_T     rows of w_g            rows of x                k           its transpose: few rows a group
+//   DX      rows of dy             columns of w_g           n           rows x k
+//   DW      columns of dy_g        columns of x_g           rows of g   n x k of group g
+//
+// "Rows" lie along the reduction axis (K-major); "columns" lie across it (MN-major): the same
+// arrays in place, no transposed copy.  A stage holds 128 bytes of the reduction axis for K-major operands
+// (64 values in 16 bits, 128 in 8, 256 in 4), or 64 of its steps as rows of 64 values for
+// MN-major ones; both with the 128-byte swizzle of the TMA load.
+//
+// The work is cut into tiles of D.  Where the groups begin is known on the device only, so every CTA
+// (one an SM) adds up the groups' tile counts once and then walks the tiles t = blockIdx.x, +
+// gridDim.x, ..., finding each tile's group by bisection.  Warp roles:
+//   warp 0      TMA loads of P and Q into the ring (full / empty barriers);
+//   warp 1      one thread issues the MMAs; tfull[a] when a tile's are done, tempty[a] before an
+//               accumulator's reuse;
+//   warps 2, 3  what the loads leave to be done, reported on fixed[s]: microscaled rows: the scales, 4 bytes
+//               of a row at a time, into the order that the tensor memory wants (row r of 128 at 16 (r % 32)
+//               + 4 (r / 32)); DW: zeros over the rows past the group's end in its last block, where the load brought the
+//               next group's rows (both operands, since a NaN times zero is none);
+//   warps 4-11  read D from tensor memory, round once and store.  Rows past the group's end and
+//               columns past the width are computed and not stored.
+// Every wait is bounded, or goes on only until another role's bounded wait has run out; then the
+// roles run out too, SMG_PROD_TIMEOUT is set, and the CTA waits (bounded) for its own copies and
+// MMAs before it frees the tensor memory.
 #pragma once
 #include "k_mx.cuh"
+#include "tc_util.cuh"
+
+enum { FORM_Y = 0, FORM_YT = 1, FORM_DX = 2, FORM_DW = 3 };
 
 struct ProdArgs {
-  const int32_t* off;
+  const int32_t* off;             // null: one group of all rows
   int n_groups, rows, n, k;
-  const void *a, *b;              // x and w | dy and w | dy and x
-  int64_t lda, ldb, b_stride;
-  const uint8_t *sa, *sb;         // scales of microscaled a and b
-  int pitch, row_bytes;
+  int p_tiles, q_tiles;           // tiles along the fixed axes (Y, YT, DX: the one in use)
+  const uint8_t *sa, *sb;         // scales of microscaled rows, and of the banks
+  int pitch;                      // bytes of a row of scales
+  uint32_t idesc;
   void* y;
   int64_t ldy, y_stride;
   int y_type;
+  bool y_vec;                     // every row of y starts on 16 bytes
   int32_t* err;
 };
 
-DEV int prod_group(const ProdArgs& g, int row) {
-  if (!g.off) return 0;
-  int f = -1;
-  for (int i = 0; i < g.n_groups; ++i)
-    if (g.off[i] <= row && row < g.off[i + 1]) f = i;
-  return f;
+#define PR_BM 128
+#define PR_THREADS 384
+#define PR_HELPERS 64
+#define PR_EPI_WARPS 8
+#define PR_SMEM_MAX 232448
+#define PR_STAGING (PR_EPI_WARPS * 2048)
+#define PR_GROUP_BYTES ((3 * SMG_PROD_MAX_GROUPS + 1) * 4)
+
+// KIND 16: f16 or bf16; 8, 4: microscaled
+template <int KIND, int BN>
+struct ProdShape {
+  static constexpr int QCH = (BN + 127) / 128;                          // 128-row parts of Q
+  static constexpr int SFW = KIND == 16 ? 0 : KIND == 8 ? 1 : 2;        // 4-byte scale words of a row and block
+  static constexpr int P_BYTES = PR_BM * 128, Q_BYTES = BN * 128, S_BYTES = (1 + QCH) * SFW * 512;
+  static constexpr int STAGE = P_BYTES + Q_BYTES + S_BYTES;
+  static constexpr int ROOM = PR_SMEM_MAX - 1024 - PR_STAGING - PR_GROUP_BYTES - 512;
+  static constexpr int STAGES = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
+  static constexpr int SMEM = STAGES * STAGE + 1024 + PR_STAGING + PR_GROUP_BYTES + 512;
+  static constexpr int SFC = (1 + QCH) * SFW * 4;                       // tensor-memory columns of a stage's scales
+  static constexpr int COLS = 2 * BN + STAGES * SFC;
+  static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static_assert(COLS <= 512 && STAGES >= 3, "tile too large");
+};
+
+DEV void pr_tma_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          ag_smem(dst)),
+      "l"((uint64_t)map), "r"(ag_smem(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
 }
 
-DEV void prod_put(const ProdArgs& g, int64_t at, float v) {
-  if (g.y_type == SMG_EMB_F32) ((float*)g.y)[at] = v;
-  else if (g.y_type == SMG_EMB_BF16) ((__nv_bfloat16*)g.y)[at] = __float2bfloat16_rn(v);
-  else ((__half*)g.y)[at] = __float2half_rn(v);
+// descriptor of an MN-major operand: 128-byte swizzle, 8-step atoms 1024 bytes apart along the
+// reduction axis, blocks of 64 values 8192 bytes apart across it
+DEV uint64_t pr_desc_mn(const void* tile) {
+  const uint32_t a = ag_smem(tile);
+  return (uint64_t)((a >> 4) & 0x3fffu) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
 }
 
-DEV void prod_check(const ProdArgs& g) {
-  if (!g.off || !g.err || blockIdx.x) return;
-  for (int i = threadIdx.x; i < g.n_groups; i += blockDim.x) {
-    const int p = g.off[i], q = g.off[i + 1];
-    if (p < 0 || q < p || q > g.rows || (i == 0 && p) || (i == g.n_groups - 1 && q != g.rows)) atomicOr(g.err, SMG_PROD_OFFSETS);
+// descriptor of 512 bytes of scales for the copy to tensor memory: no swizzle, 8-row parts 128 bytes apart
+DEV uint64_t pr_desc_scales(const void* p) {
+  const uint32_t a = ag_smem(p);
+  return (uint64_t)((a >> 4) & 0x3fffu) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+
+DEV void pr_mma16(uint32_t d, uint64_t p, uint64_t q, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(p), "l"(q), "r"(idesc), "r"(accum));
+}
+
+template <int KIND>
+DEV void pr_mma_mx(uint32_t d, uint64_t p, uint64_t q, uint32_t idesc, uint32_t sp, uint32_t sq, uint32_t accum) {
+  if constexpr (KIND == 4)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(p), "l"(q), "r"(idesc), "r"(sp), "r"(sq), "r"(accum));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(p), "l"(q), "r"(idesc), "r"(sp), "r"(sq), "r"(accum));
+}
+
+DEV void pr_copy_scales(uint32_t tmem, const void* p) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(pr_desc_scales(p)) : "memory");
+}
+
+DEV void pr_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+DEV void pr_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ag_smem(b)) : "memory"); }
+
+// A wait that may rightly last as long as a whole tile: it goes on while no role has failed (their
+// own waits are bounded).
+DEV bool pr_wait_long(uint64_t* b, uint32_t parity, volatile int* failed) {
+  while (!ag_wait(b, parity))
+    if (*failed) return false;
+  return true;
+}
+
+// what every role knows of the tiles
+struct ProdTiles {
+  const int *beg, *end, *cum;   // first row, row past the last, and first row tile of each group
+  int n_groups, fixed;          // tiles of a row tile along the fixed axes
+  int total;
+};
+
+struct ProdTile {
+  int g, r0, r1;                // group, first row of the tile, row past the group's last
+  int f;                        // index along the fixed axes
+};
+
+template <int FORM, int BN>
+DEV ProdTile prod_tile(const ProdTiles& T, int t) {
+  const int u = t / T.fixed;
+  int lo = 0, hi = T.n_groups;  // the last group whose first row tile is <= u (empty groups have none)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (T.cum[mid] <= u) lo = mid;
+    else hi = mid;
   }
+  ProdTile r;
+  r.g = lo;
+  r.f = t - u * T.fixed;
+  r.r0 = T.beg[lo] + (FORM == FORM_DW ? 0 : (u - T.cum[lo]) * (FORM == FORM_YT ? BN : PR_BM));
+  r.r1 = T.end[lo];
+  return r;
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(256) k_prod_y(ProdArgs g) {
-  typedef typename Elem<TYPE>::T T;
-  prod_check(g);
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)g.rows * g.n; t += (int64_t)gridDim.x * 256) {
-    const int row = (int)(t / g.n), j = (int)(t % g.n), q = prod_group(g, row);
-    if (q < 0) continue;
-    const T *a = (const T*)g.a + row * g.lda, *b = (const T*)g.b + q * g.b_stride + j * g.ldb;
-    float s = 0.f;
-    for (int i = 0; i < g.k; ++i) s = __fmaf_rn(Elem<TYPE>::up(a[i]), Elem<TYPE>::up(b[i]), s);
-    prod_put(g, row * g.ldy + j, s);
-  }
-}
+template <int KIND, int BN, int FORM>
+__global__ void __launch_bounds__(PR_THREADS, 1)
+    k_prod(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ ProdArgs g) {
+  using S = ProdShape<KIND, BN>;
+  constexpr int STAGES = S::STAGES;
+  constexpr bool P_MN = FORM == FORM_DW, Q_MN = FORM == FORM_DX || FORM == FORM_DW;
+  constexpr int BK = P_MN || Q_MN ? 64 : 1024 / KIND;   // values of the reduction axis in a stage
+  constexpr int SUB = BK / 4;                           // and in an MMA
+  constexpr bool HELP = KIND != 16 || FORM == FORM_DW;
+  extern __shared__ unsigned char pr_raw[];
+  unsigned char* base = (unsigned char*)(((uintptr_t)pr_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* sP = base;
+  unsigned char* sQ = sP + STAGES * S::P_BYTES;
+  unsigned char* sS = sQ + STAGES * S::Q_BYTES;
+  unsigned char* staging = sS + STAGES * S::S_BYTES;
+  int* s_beg = (int*)(staging + PR_STAGING);
+  int* s_end = s_beg + SMG_PROD_MAX_GROUPS;
+  int* s_cum = s_end + SMG_PROD_MAX_GROUPS;
+  uint64_t* full = (uint64_t*)(((uintptr_t)(s_cum + SMG_PROD_MAX_GROUPS + 1) + 7) & ~(uintptr_t)7);
+  uint64_t* empty = full + STAGES;
+  uint64_t* fixed = empty + STAGES;
+  uint64_t* tfull = fixed + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* done = tempty + 2;
+  uint32_t* tmem_slot = (uint32_t*)(done + 1);
+  __shared__ int sh_fail;
+  volatile int* failed = &sh_fail;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-template <int TYPE>
-__global__ void __launch_bounds__(256) k_prod_dx(ProdArgs g) {
-  typedef typename Elem<TYPE>::T T;
-  prod_check(g);
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)g.rows * g.k; t += (int64_t)gridDim.x * 256) {
-    const int row = (int)(t / g.k), i = (int)(t % g.k), q = prod_group(g, row);
-    if (q < 0) continue;
-    const T *a = (const T*)g.a + row * g.lda, *b = (const T*)g.b + q * g.b_stride + i;
-    float s = 0.f;
-    for (int j = 0; j < g.n; ++j) s = __fmaf_rn(Elem<TYPE>::up(a[j]), Elem<TYPE>::up(b[j * g.ldb]), s);
-    prod_put(g, row * g.ldy + i, s);
-  }
-}
-
-template <int TYPE>
-__global__ void __launch_bounds__(256) k_prod_dw(ProdArgs g) {
-  typedef typename Elem<TYPE>::T T;
-  prod_check(g);
-  const int64_t per = (int64_t)g.n * g.k;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < per * g.n_groups; t += (int64_t)gridDim.x * 256) {
-    const int q = (int)(t / per), j = (int)(t % per / g.k), i = (int)(t % g.k);
-    int r0 = g.off ? g.off[q] : 0, r1 = g.off ? g.off[q + 1] : g.rows;
-    if (r0 < 0 || r1 < r0 || r1 > g.rows) r1 = r0 = 0;
-    float s = 0.f;
-    for (int64_t r = r0; r < r1; ++r)
-      s = __fmaf_rn(Elem<TYPE>::up(((const T*)g.a)[r * g.lda + j]), Elem<TYPE>::up(((const T*)g.b)[r * g.ldb + i]), s);
-    prod_put(g, q * g.y_stride + j * g.ldy + i, s);
-  }
-}
-
-template <int BITS>
-__global__ void __launch_bounds__(256) k_prod_mx(ProdArgs g) {
-  prod_check(g);
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)g.rows * g.n; t += (int64_t)gridDim.x * 256) {
-    const int row = (int)(t / g.n), j = (int)(t % g.n), q = prod_group(g, row);
-    if (q < 0) continue;
-    const int64_t br = (int64_t)q * g.n + j;
-    float s = 0.f;
-    for (int v = 0; v < g.row_bytes / BITS; ++v) {   // 8 values are BITS bytes
-      uint32_t c[2] = {0, 0}, d[2] = {0, 0};
-      const uint32_t* p = (const uint32_t*)((const uint8_t*)g.a + (int64_t)row * g.row_bytes + v * BITS);
-      const uint32_t* w = (const uint32_t*)((const uint8_t*)g.b + br * g.row_bytes + v * BITS);
-#pragma unroll
-      for (int i = 0; i < BITS / 4; ++i) { c[i] = p[i]; d[i] = w[i]; }
-      float x[8], y[8], e = 0.f;
-      mx_decode<BITS>(c, x);
-      mx_decode<BITS>(d, y);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e = __fmaf_rn(x[i], y[i], e);
-      const int sx = g.sa[(int64_t)row * g.pitch + (v >> 2)], sy = g.sb[br * g.pitch + (v >> 2)];
-      s += sx == 255 || sy == 255 ? __int_as_float(0x7fc00000) : e * mx_two(sx - 127) * mx_two(sy - 127);
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      ag_mbar_init(&full[s], 1);
+      ag_mbar_init(&empty[s], 1);
+      ag_mbar_init(&fixed[s], KIND == 16 ? PR_HELPERS / 32 : PR_HELPERS);
     }
-    prod_put(g, row * g.ldy + j, s);
+    for (int a = 0; a < 2; ++a) {
+      ag_mbar_init(&tfull[a], 1);
+      ag_mbar_init(&tempty[a], PR_EPI_WARPS);
+    }
+    ag_mbar_init(done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    sh_fail = 0;
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ag_smem(tmem_slot)), "r"(S::TMEM)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // groups: offsets that break the rules are reported, and every group is then taken as empty
+  int bad = 0;
+  for (int i = tid; i < g.n_groups; i += PR_THREADS) {
+    int a = 0, b = g.rows;
+    if (g.off) {
+      a = g.off[i];
+      b = g.off[i + 1];
+      bad |= a < 0 || b < a || b > g.rows || (i == 0 && a != 0) || (i == g.n_groups - 1 && b != g.rows);
+    }
+    s_beg[i] = a;
+    s_end[i] = b;
+  }
+  ag_fence_before();
+  bad = __syncthreads_or(bad);
+  ag_fence_after();
+  if (bad) {
+    if (tid == 0 && blockIdx.x == 0 && g.err) atomicOr(g.err, SMG_PROD_OFFSETS);
+    for (int i = tid; i < g.n_groups; i += PR_THREADS) s_beg[i] = s_end[i] = 0;
+    __syncthreads();
+  }
+  const uint32_t tmem = *tmem_slot;
+  constexpr int RT = FORM == FORM_YT ? BN : PR_BM;
+  if (warp == 0) {   // first row tile of every group
+    int at = 0;
+    for (int i0 = 0; i0 < g.n_groups; i0 += 32) {
+      const int i = i0 + lane;
+      const int own = i >= g.n_groups ? 0 : FORM == FORM_DW ? 1 : (s_end[i] - s_beg[i] + RT - 1) / RT;
+      int sum = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      if (i < g.n_groups) s_cum[i] = at + sum - own;
+      at += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) s_cum[g.n_groups] = at;
+  }
+  __syncthreads();
+  ProdTiles T;
+  T.beg = s_beg; T.end = s_end; T.cum = s_cum;
+  T.n_groups = g.n_groups;
+  T.fixed = FORM == FORM_DW ? g.p_tiles * g.q_tiles : FORM == FORM_YT ? g.p_tiles : g.q_tiles;
+  T.total = s_cum[g.n_groups] * T.fixed;
+  const int red = FORM == FORM_DX ? g.n : g.k;   // (DW: the group's rows)
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {   // loads
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x) {
+        const ProdTile c = prod_tile<FORM, BN>(T, t);
+        const int nk = ((FORM == FORM_DW ? c.r1 - c.r0 : red) + BK - 1) / BK;
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const int s = (int)(it % STAGES);
+          if (it >= STAGES && !ag_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
+          unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
+          ag_expect_tx(&full[s], S::P_BYTES + S::Q_BYTES);
+          const int x = KIND == 16 ? kb * BK : kb * 128;   // microscaled rows are loaded as bytes
+          if (FORM == FORM_Y) {
+            ag_tma_2d(&tmA, &full[s], p, x, c.r0);
+            pr_tma_3d(&tmB, &full[s], q, x, c.f * BN, c.g);
+          } else if (FORM == FORM_YT) {
+            pr_tma_3d(&tmB, &full[s], p, x, c.f * PR_BM, c.g);
+            ag_tma_2d(&tmA, &full[s], q, x, c.r0);
+          } else if (FORM == FORM_DX) {
+            ag_tma_2d(&tmA, &full[s], p, x, c.r0);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) pr_tma_3d(&tmB, &full[s], q + j * 8192, c.f * BN + j * 64, x, c.g);
+          } else {
+            const int m0 = c.f % g.p_tiles * PR_BM, n0 = c.f / g.p_tiles * BN;
+#pragma unroll
+            for (int j = 0; j < PR_BM / 64; ++j) ag_tma_2d(&tmA, &full[s], p + j * 8192, m0 + j * 64, c.r0 + x);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) ag_tma_2d(&tmB, &full[s], q + j * 8192, n0 + j * 64, c.r0 + x);
+          }
+        }
+      }
+      // the last loads must have landed before the CTA ends
+      const uint32_t first = it > STAGES ? it - STAGES : 0;
+      for (uint32_t j = first; j < it; ++j) ok = ag_wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
+      if (!ok) *failed = 1;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {   // MMAs
+      uint32_t it = 0, j = 0;
+      for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x, ++j) {
+        const ProdTile c = prod_tile<FORM, BN>(T, t);
+        const int len = FORM == FORM_DW ? c.r1 - c.r0 : red, nk = (len + BK - 1) / BK;
+        const uint32_t acc = j & 1u;
+        if (j >= 2 && !ag_wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
+        ag_fence_after();
+        const uint32_t d = tmem + acc * BN;
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const int s = (int)(it % STAGES);
+          const uint32_t ph = (it / STAGES) & 1u;
+          const int left = len - kb * BK;
+          if (!ag_wait(&full[s], ph)) { ok = false; break; }
+          if (HELP && !ag_wait(&fixed[s], ph)) { ok = false; break; }
+          if (KIND != 16) pr_proxy_fence();   // the scales were written by ordinary copies
+          ag_fence_after();
+          const unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
+          const uint64_t dp = P_MN ? pr_desc_mn(p) : ag_desc(p), dq = Q_MN ? pr_desc_mn(q) : ag_desc(q);
+          const int subs = left >= BK ? 4 : (left + SUB - 1) / SUB;
+          if constexpr (KIND == 16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (i < subs) pr_mma16(d, dp + i * (P_MN ? 128 : 2), dq + i * (Q_MN ? 128 : 2), g.idesc, (kb | i) != 0);
+          } else {
+            const unsigned char* sc = sS + s * S::S_BYTES;
+            const uint32_t tp = tmem + 2 * BN + s * S::SFC, tq = tp + S::SFW * 4;
+#pragma unroll
+            for (int i = 0; i < S::SFW; ++i) pr_copy_scales(tp + 4 * i, sc + 512 * i);
+#pragma unroll
+            for (int i = 0; i < S::SFW * S::QCH; ++i) pr_copy_scales(tq + 4 * i, sc + 512 * (S::SFW + i));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (i < subs) {
+                // an MMA's 2 scales of a row (e2m1) are half a word, its one (e4m3) is a byte of it
+                const uint32_t w = KIND == 4 ? i / 2 : 0, id = KIND == 4 ? (i & 1) * 2 : i;
+                pr_mma_mx<KIND>(d, dp + i * 2, dq + i * 2, g.idesc | id << 29 | id << 4, tp + 4 * w, tq + 4 * S::QCH * w, (kb | i) != 0);
+              }
+            }
+          }
+          ag_commit(&empty[s]);
+        }
+        ag_commit(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
+      }
+      ag_commit(done);   // every issued MMA has completed before the tensor memory is freed
+      if (!ag_wait(done, 0) || !ok) *failed = 1;
+    }
+  } else if (warp < 4) {
+    if (HELP) {
+      const int h = tid - 64;
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x) {
+        const ProdTile c = prod_tile<FORM, BN>(T, t);
+        if constexpr (KIND != 16) {
+          const int nk = (red + BK - 1) / BK;
+          // rows of w_g and rows of x, whichever is P
+          const int w0 = c.f * (FORM == FORM_YT ? PR_BM : BN);
+          const int p_lim = FORM == FORM_YT ? g.n - w0 : c.r1 - c.r0, q_lim = FORM == FORM_YT ? c.r1 - c.r0 : g.n - w0;
+          const int64_t wr = (int64_t)c.g * g.n + w0, xr = c.r0;
+          const uint8_t* ps = (FORM == FORM_YT ? g.sb + wr * g.pitch : g.sa + xr * g.pitch);
+          const uint8_t* qs = (FORM == FORM_YT ? g.sa + xr * g.pitch : g.sb + wr * g.pitch);
+          for (int kb = 0; kb < nk; ++kb, ++it) {
+            const int s = (int)(it % STAGES);
+            if (it >= STAGES && !ag_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
+            const uint32_t sc = ag_smem(sS + s * S::S_BYTES);
+#pragma unroll
+            for (int w = 0; w < S::SFW; ++w) {
+              const int col = (kb * S::SFW + w) * 4;
+#pragma unroll
+              for (int r0 = 0; r0 < PR_BM + BN; r0 += PR_HELPERS) {
+                const int rr = r0 + h, r = rr < PR_BM ? rr : rr - PR_BM;
+                if (rr >= PR_BM + BN) break;
+                const bool is_p = rr < PR_BM;
+                const bool live = col < g.pitch && r < (is_p ? p_lim : q_lim);
+                const uint8_t* src = live ? (is_p ? ps : qs) + (int64_t)r * g.pitch + col : g.sa;
+                const uint32_t part = is_p ? w : S::SFW + w * S::QCH + (r >> 7);
+                const uint32_t dst = sc + 512 * part + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+              }
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ag_smem(&fixed[s])) : "memory");
+          }
+        } else {
+          const int len = c.r1 - c.r0;
+          // every block is passed on, whole or not: a wait that skipped blocks could not tell a
+          // stage's next filling from the one after
+          for (int k0 = 0; k0 < len; k0 += BK, ++it) {
+            const int s = (int)(it % STAGES), tail = len - k0;
+            if (!__all_sync(0xffffffffu, pr_wait_long(&full[s], (it / STAGES) & 1u, failed))) { ok = false; break; }
+            if (tail < BK) {
+              // steps tail .. 63 of every block of 64 values: 128 bytes each, the swizzle stays within them
+              for (int i = h; i < (PR_BM + BN) / 64 * (BK - tail) * 8; i += PR_HELPERS) {
+                const int v = i & 7, step = tail + (i >> 3) % (BK - tail), b = (i >> 3) / (BK - tail);
+                unsigned char* z = b < PR_BM / 64 ? sP + s * S::P_BYTES + b * 8192 : sQ + s * S::Q_BYTES + (b - PR_BM / 64) * 8192;
+                *(uint4*)(z + step * 128 + v * 16) = make_uint4(0, 0, 0, 0);
+              }
+              pr_proxy_fence();
+            }
+            __syncwarp();
+            if (lane == 0) pr_arrive(&fixed[s]);
+          }
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (!ok) *failed = 1;
+    }
+  } else {   // results
+    const int ew = warp - 4, quarter = ew & 3, half = ew >> 2;
+    unsigned char* stg = staging + ew * 2048;
+    uint32_t j = 0;
+    for (int t = blockIdx.x; t < T.total; t += gridDim.x, ++j) {
+      const ProdTile c = prod_tile<FORM, BN>(T, t);
+      const uint32_t acc = j & 1u;
+      if (!__all_sync(0xffffffffu, pr_wait_long(&tfull[acc], (j >> 1) & 1u, failed) && !*failed)) {
+        if (lane == 0) *failed = 1;
+        break;
+      }
+      ag_fence_after();
+      const bool none = FORM == FORM_DW && c.r1 == c.r0;   // an empty group: zeros
+      const uint32_t d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
+      // tile's place in y: rows row0 .. row_lim - 1, columns col0 .. col_lim - 1
+      const int row0 = FORM == FORM_DW ? c.f % g.p_tiles * PR_BM : c.r0, row_lim = FORM == FORM_DW ? g.n : c.r1;
+      const int col0 = FORM == FORM_DW ? c.f / g.p_tiles * BN : c.f * (FORM == FORM_YT ? PR_BM : BN);
+      const int col_lim = FORM == FORM_Y || FORM == FORM_YT ? g.n : g.k;
+      const int64_t y0 = FORM == FORM_DW ? (int64_t)c.g * g.y_stride : 0;
+      constexpr int HALF = BN >= 64 ? BN / 2 : BN;         // columns of D that a warp takes
+      if (BN >= 64 || half == 0) {
+        for (int c0 = half * HALF; c0 < half * HALF + HALF; c0 += 32) {
+          if (FORM == FORM_YT) {
+            if (row0 + c0 >= row_lim) break;
+          } else if (col0 + c0 >= col_lim) {
+            break;
+          }
+          uint32_t v[32];
+          if (none) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0;
+          } else {
+            ag_tmem_ld32(d + c0, v);
+          }
+          if (FORM == FORM_YT) {   // lane: a column of y; v[i]: row row0 + c0 + i
+            const int col = col0 + quarter * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int row = row0 + c0 + i;
+              if (row < row_lim && col < col_lim) {
+                const int64_t at = (int64_t)row * g.ldy + col;
+                const float f = __uint_as_float(v[i]);
+                if (g.y_type == SMG_EMB_F32) ((float*)g.y)[at] = f;
+                else if (g.y_type == SMG_EMB_BF16) ((__nv_bfloat16*)g.y)[at] = __float2bfloat16_rn(f);
+                else ((__half*)g.y)[at] = __float2half_rn(f);
+              }
+            }
+          } else {
+            // through shared memory: rows of 64 bytes (32 values of 16 bits, or 16 of 32), 16-byte parts swapped about by the
+            // row, so that both a lane's own row and 8 rows side by side meet no bank twice
+            const int per = g.y_type == SMG_EMB_F32 ? 16 : 32;
+            for (int h0 = 0; h0 < 32; h0 += per) {
+              uint32_t w[16];
+              if (g.y_type == SMG_EMB_F32) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = h0 ? v[16 + i] : v[i];
+              } else if (g.y_type == SMG_EMB_BF16) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                  w[i] = *(const uint32_t*)&b;
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const __half2 b = __floats2half2_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                  w[i] = *(const uint32_t*)&b;
+                }
+              }
+              __syncwarp();
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *(uint4*)(stg + lane * 64 + ((q ^ (lane >> 1)) & 3) * 16) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+              __syncwarp();
+              const int size = g.y_type == SMG_EMB_F32 ? 4 : 2, each = 16 / size;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (lane >> 2), q = lane & 3;
+                const int row = row0 + quarter * 32 + r, col = col0 + c0 + h0 + q * each;
+                if (row >= row_lim || col >= col_lim) continue;
+                const uint4 u = *(const uint4*)(stg + r * 64 + ((q ^ (r >> 1)) & 3) * 16);
+                unsigned char* o = (unsigned char*)g.y + (y0 + (int64_t)row * g.ldy + col) * size;
+                if (g.y_vec && col + each <= col_lim) {
+                  *(uint4*)o = u;
+                } else {
+                  const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) {
+                    if (e >= each || col + e >= col_lim) break;
+                    if (size == 4) ((uint32_t*)o)[e] = uw[e & 3];
+                    else ((uint16_t*)o)[e] = (uint16_t)(uw[e >> 1] >> (16 * (e & 1)));
+                  }
+                }
+              }
+            }
+          }
+        }
+      }
+      ag_fence_before();
+      __syncwarp();
+      if (lane == 0) pr_arrive(&tempty[acc]);
+    }
+  }
+  __syncwarp();
+  ag_fence_before();
+  __syncthreads();
+  if (tid == 0 && *failed && g.err) atomicOr(g.err, SMG_PROD_TIMEOUT);
+  if (warp == 2) {
+    ag_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
   }
 }

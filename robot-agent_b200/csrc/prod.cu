@@ -4,10 +4,16 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <algorithm>
+#include <atomic>
+
 #include "k_norm.cuh"
 #include "k_prod.cuh"
 
-int smg_set_error(int code, const char* msg);   // smg.cu: records msg for smg_last_error
+#include <cudaTypedefs.h>
+
+int smg_set_error(int code, const char* msg);              // smg.cu: records msg for smg_last_error
+extern "C" PFN_cuTensorMapEncodeTiled_v12000 smg_tmap_encoder();   // smg.cu
 
 static int fail(int code, const char* fmt, ...) {
   char msg[256];
@@ -54,19 +60,87 @@ static int out_rows(const char* who, const void* p, int64_t ld, int64_t len, int
   return SMG_OK;
 }
 
-static ProdArgs prod_fill(const int32_t* off, int n_groups, int rows, int n, int k, const void* a, int64_t lda, const void* b, int64_t ldb,
-                          int64_t b_stride, void* y, int64_t ldy, int64_t y_stride, int y_type, int32_t* err) {
+// SMs of the current device
+static int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Rows for the tensor-core loads: `outer` groups of `rows` rows of `len` values (microscaled rows: bytes),
+// boxes of 128 bytes x box_rows, 128-byte swizzle, zeros outside the array.
+static int encode(const char* who, CUtensorMap* m, const void* p, bool bytes, int64_t len, int64_t rows, int64_t outer, int64_t ld,
+                  int64_t outer_stride, int box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = smg_tmap_encoder();
+  if (!fn) return fail(SMG_ERR_DEVICE, "%s: cuTensorMapEncodeTiled unavailable", who);
+  const int size = bytes ? 1 : 2;
+  const cuuint64_t dim[3] = {(cuuint64_t)len, (cuuint64_t)std::max<int64_t>(rows, 1), (cuuint64_t)std::max<int64_t>(outer, 1)};
+  const cuuint64_t str[2] = {(cuuint64_t)ld * size, (cuuint64_t)outer_stride * size};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
+  const cuuint32_t est[3] = {1, 1, 1};
+  const CUresult r = fn(m, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, outer ? 3 : 2, const_cast<void*>(p),
+                        dim, str, box, est, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SMG_ERR_ARGS, "%s: tensor map refused (%d): a row or group is too far from the next", who, (int)r);
+  return SMG_OK;
+}
+
+// A product's operands: A has the packed rows, B the groups' fixed rows (DW: the packed rows of x)
+struct Operands {
+  const void *a, *b;
+  int64_t lda, ldb, b_stride;
+  int64_t a_len, b_len;   // values of a row (microscaled: bytes)
+};
+
+template <int KIND, int BN, int FORM>
+static int launch(const char* who, const Operands& o, ProdArgs g, int type, cudaStream_t st) {
+  using S = ProdShape<KIND, BN>;
+  constexpr bool bytes = KIND != 16;
+  const int wide = FORM == FORM_Y || FORM == FORM_YT ? g.n : g.k;
+  g.p_tiles = FORM == FORM_YT ? (g.n + PR_BM - 1) / PR_BM : FORM == FORM_DW ? (g.n + PR_BM - 1) / PR_BM : 1;
+  g.q_tiles = FORM == FORM_YT ? 1 : (wide + BN - 1) / BN;
+  const int64_t per = (int64_t)g.p_tiles * g.q_tiles, rt = FORM == FORM_YT ? BN : PR_BM;
+  const int64_t row_tiles = FORM == FORM_DW ? g.n_groups : g.rows / rt + std::min(g.n_groups, g.rows);   // at most
+  if (row_tiles * per > 0x7fffffff) return fail(SMG_ERR_CAPACITY, "%s: too many tiles for one call", who);
+  CUtensorMap tA, tB;
+  int r;
+  if (FORM == FORM_DW) {
+    r = encode(who, &tA, o.a, bytes, o.a_len, g.rows, 0, o.lda, 0, 64);
+    if (!r) r = encode(who, &tB, o.b, bytes, o.b_len, g.rows, 0, o.ldb, 0, 64);
+  } else {
+    r = encode(who, &tA, o.a, bytes, o.a_len, g.rows, 0, o.lda, 0, FORM == FORM_YT ? BN : PR_BM);
+    if (!r) r = encode(who, &tB, o.b, bytes, o.b_len, g.n, g.n_groups, o.ldb, g.n_groups > 1 ? o.b_stride : o.ldb * (int64_t)g.n,
+                       FORM == FORM_Y ? BN : FORM == FORM_YT ? PR_BM : 64);
+  }
+  if (r) return r;
+  // instruction descriptor: operand types (f16 0, bf16 1 with 32-bit sums in bits 4-5; e4m3 0, e2m1 1 with
+  // power-of-two scales in bit 23) at 7 and 10, MN-major P and Q at 15 and 16, BN / 8 at 17, 128 / 16 at 24
+  const uint32_t fmt = KIND == 16 ? (type == SMG_EMB_BF16) : KIND == 4;
+  g.idesc = fmt << 7 | fmt << 10 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(PR_BM >> 4) << 24 | (KIND == 16 ? 1u << 4 : 1u << 23) |
+            (FORM == FORM_DW ? 1u << 15 : 0u) | (FORM == FORM_DX || FORM == FORM_DW ? 1u << 16 : 0u);
+  g.y_vec = rows16(g.y, g.ldy, g.y_type) && (FORM != FORM_DW || g.y_stride * size_of(g.y_type) % 16 == 0);
+  const int sms = sm_count();
+  const cudaError_t e = cudaFuncSetAttribute(k_prod<KIND, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  if (!sms || e != cudaSuccess) return fail(SMG_ERR_DEVICE, "%s: no usable device (%s)", who, cudaGetErrorString(cudaGetLastError()));
+  k_prod<KIND, BN, FORM><<<(unsigned)std::min<int64_t>(sms, row_tiles * per), PR_THREADS, S::SMEM, st>>>(tA, tB, g);
+  return launched(who);
+}
+
+static ProdArgs prod_fill(const int32_t* off, int n_groups, int rows, int n, int k, void* y, int64_t ldy, int64_t y_stride, int y_type,
+                          int32_t* err) {
   ProdArgs g = {};
   g.off = off; g.n_groups = n_groups; g.rows = rows; g.n = n; g.k = k;
-  g.a = a; g.lda = lda; g.b = b; g.ldb = ldb; g.b_stride = b_stride;
   g.y = y; g.ldy = ldy; g.y_stride = y_stride; g.y_type = y_type; g.err = err;
   return g;
 }
 
-static int grid_for(int64_t threads) {
-  const int64_t b = (threads + 255) / 256;
-  return (int)(b < 1 ? 1 : b > 148 * 64 ? 148 * 64 : b);
-}
+// Few rows a group: their tile is the narrow side (FORM_YT), so that the MMAs are not mostly over rows
+// that are not there.
+static bool few_rows(int rows, int n_groups) { return (int64_t)rows <= 32ll * n_groups; }
 
 extern "C" {
 
@@ -80,11 +154,10 @@ int smg_group_product(const void* x, int64_t ldx, const void* w, int64_t ldw, in
     if (int r = operand(who, "w (from group to group)", w, w_stride, (int64_t)(n - 1) * ldw + k, n)) return r;
   if (int r = out_rows(who, y, ldy, n, rows)) return r;
   if (rows == 0) return SMG_OK;
-  const ProdArgs g = prod_fill(off, n_groups, rows, n, k, x, ldx, w, ldw, w_stride, y, ldy, 0, y_type, err);
-  const int grid = grid_for((int64_t)rows * n);
-  if (type == SMG_EMB_BF16) k_prod_y<SMG_EMB_BF16><<<grid, 256, 0, (cudaStream_t)stream>>>(g);
-  else k_prod_y<SMG_EMB_F16><<<grid, 256, 0, (cudaStream_t)stream>>>(g);
-  return launched(who);
+  const ProdArgs g = prod_fill(off, n_groups, rows, n, k, y, ldy, 0, y_type, err);
+  const Operands o = {x, w, ldx, ldw, w_stride, k, k};
+  if (few_rows(rows, n_groups)) return launch<16, 32, FORM_YT>(who, o, g, type, (cudaStream_t)stream);
+  return launch<16, 256, FORM_Y>(who, o, g, type, (cudaStream_t)stream);
 }
 
 int smg_group_product_dx(const void* dy, int64_t lddy, const void* w, int64_t ldw, int64_t w_stride, const int32_t* off,
@@ -98,11 +171,9 @@ int smg_group_product_dx(const void* dy, int64_t lddy, const void* w, int64_t ld
     if (int r = operand(who, "w (from group to group)", w, w_stride, (int64_t)(n - 1) * ldw + k, n)) return r;
   if (int r = out_rows(who, dx, lddx, k, rows)) return r;
   if (rows == 0) return SMG_OK;
-  const ProdArgs g = prod_fill(off, n_groups, rows, n, k, dy, lddy, w, ldw, w_stride, dx, lddx, 0, dx_type, err);
-  const int grid = grid_for((int64_t)rows * k);
-  if (type == SMG_EMB_BF16) k_prod_dx<SMG_EMB_BF16><<<grid, 256, 0, (cudaStream_t)stream>>>(g);
-  else k_prod_dx<SMG_EMB_F16><<<grid, 256, 0, (cudaStream_t)stream>>>(g);
-  return launched(who);
+  const ProdArgs g = prod_fill(off, n_groups, rows, n, k, dx, lddx, 0, dx_type, err);
+  const Operands o = {dy, w, lddy, ldw, w_stride, n, k};
+  return launch<16, 256, FORM_DX>(who, o, g, type, (cudaStream_t)stream);
 }
 
 int smg_group_product_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int32_t* off, int n_groups, int rows,
@@ -114,11 +185,15 @@ int smg_group_product_dw(const void* dy, int64_t lddy, const void* x, int64_t ld
   if (int r = operand(who, "x", x, ldx, k, rows)) return r;
   if (int r = out_rows(who, dw, lddw, k, n)) return r;
   if (n_groups > 1 && dw_stride < (int64_t)(n - 1) * lddw + k) return fail(SMG_ERR_ARGS, "%s: the groups of dw overlap", who);
-  const ProdArgs g = prod_fill(off, n_groups, rows, n, k, dy, lddy, x, ldx, 0, dw, lddw, dw_stride, dw_type, err);
-  const int grid = grid_for((int64_t)n_groups * n * k);
-  if (type == SMG_EMB_BF16) k_prod_dw<SMG_EMB_BF16><<<grid, 256, 0, (cudaStream_t)stream>>>(g);
-  else k_prod_dw<SMG_EMB_F16><<<grid, 256, 0, (cudaStream_t)stream>>>(g);
-  return launched(who);
+  ProdArgs g = prod_fill(off, n_groups, rows, n, k, dw, lddw, dw_stride, dw_type, err);
+  Operands o = {dy, x, lddy, ldx, 0, n, k};
+  if (rows == 0) {   // every group is empty and nothing is loaded: dw itself stands in for the operands
+    if (!on16(dw)) return fail(SMG_ERR_ARGS, "%s: without rows dw must start on 16 bytes", who);
+    o.a = o.b = dw;
+    o.lda = (n + 7) / 8 * 8;
+    o.ldb = (k + 7) / 8 * 8;
+  }
+  return launch<16, 256, FORM_DW>(who, o, g, type, (cudaStream_t)stream);
 }
 
 // ------------------------------------------------------------------ microscaled rows
@@ -203,13 +278,15 @@ int smg_mx_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_
   if (int r = out_rows(who, y, ldy, n, rows)) return r;
   if (rows == 0) return SMG_OK;
   if (!a_codes || !b_codes) return fail(SMG_ERR_ARGS, "%s: no codes", who);
-  ProdArgs g = prod_fill(off, n_groups, rows, n, k, a_codes, 0, b_codes, 0, 0, y, ldy, 0, y_type, err);
-  const MxOut o = mx_rows(k, nullptr, nullptr, nullptr);
-  g.sa = a_scales; g.sb = b_scales; g.pitch = o.pitch; g.row_bytes = o.kb * 4 * bits;
-  const int grid = grid_for((int64_t)rows * n);
-  if (bits == 4) k_prod_mx<4><<<grid, 256, 0, (cudaStream_t)stream>>>(g);
-  else k_prod_mx<8><<<grid, 256, 0, (cudaStream_t)stream>>>(g);
-  return launched(who);
+  ProdArgs g = prod_fill(off, n_groups, rows, n, k, y, ldy, 0, y_type, err);
+  const MxOut m = mx_rows(k, nullptr, nullptr, nullptr);
+  g.sa = a_scales; g.sb = b_scales; g.pitch = m.pitch;
+  const int64_t len = (int64_t)m.kb * 4 * bits;
+  const Operands o = {a_codes, b_codes, len, len, len * n, len, len};
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (few_rows(rows, n_groups))
+    return bits == 4 ? launch<4, 32, FORM_YT>(who, o, g, 0, st) : launch<8, 32, FORM_YT>(who, o, g, 0, st);
+  return bits == 4 ? launch<4, 192, FORM_Y>(who, o, g, 0, st) : launch<8, 192, FORM_Y>(who, o, g, 0, st);
 }
 
 // ------------------------------------------------------------------ residual norm

@@ -2013,7 +2013,7 @@ struct smg_assoc {
   int n_sm = 148;
 };
 
-static PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
+__attribute__((visibility("hidden"))) PFN_cuTensorMapEncodeTiled_v12000 smg_tmap_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -2028,7 +2028,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
 
 // 2D bf16 [rows][dim] K-major, box = 64 x box_rows, 128-byte swizzle, zero fill outside
 static int encode_rows(CUtensorMap* m, const void* ptr, int rows, int dim, int box_rows) {
-  PFN_cuTensorMapEncodeTiled_v12000 fn = tmap_encoder();
+  PFN_cuTensorMapEncodeTiled_v12000 fn = smg_tmap_encoder();
   if (!fn) return fail(SMG_ERR_DEVICE, "smg_assoc: cuTensorMapEncodeTiled unavailable");
   const cuuint64_t gdim[2] = {(cuuint64_t)dim, (cuuint64_t)rows};
   const cuuint64_t gstr[1] = {(cuuint64_t)dim * 2};

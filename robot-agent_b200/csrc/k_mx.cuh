@@ -59,6 +59,25 @@ DEV void load8(const typename Elem<TYPE>::T* p, int n, bool vec, float (&v)[8]) 
   }
 }
 
+// The same in two steps, for kernels that first issue all of a row's loads: 8 values as they lie in
+// memory (none past n: zero bits are the value 0), and the floats they are.  VEC: p on 16 bytes, n a multiple of 8.
+template <int TYPE>
+struct Raw8 {
+  typedef typename Elem<TYPE>::T T;
+  union { uint4 q[sizeof(T) / 2]; T t[8]; };
+  template <bool VEC>
+  DEV void load(const T* p, int n) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = n > 0 ? __ldg((const uint4*)p + i) : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = i < n ? p[i] : Elem<TYPE>::down(0.f);
+    }
+  }
+  DEV float get(int i) const { return Elem<TYPE>::up(t[i]); }
+};
+
 template <int TYPE>
 DEV void store8(typename Elem<TYPE>::T* p, int n, bool vec, const float (&v)[8]) {
   typedef typename Elem<TYPE>::T T;
@@ -184,39 +203,70 @@ DEV void mx_emit(const MxOut& o, int64_t row, int j, const float (&v)[8]) {
   }
 }
 
-// One thread per 8 values.  Bound by memory: per value it reads the input once and writes
-// bits / 8 + 1/32 bytes (and 2 with `values`).
-template <int TYPE, int BITS>
-__global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::T* x, int64_t ldx, int64_t n, bool vec, MxOut o) {
-  const int per = o.pitch * 4;   // threads a row
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = t / per;
-  const int j = (int)(t - row * per);
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (t < n) load8<TYPE>(x + row * ldx + 8 * j, o.dim - 8 * j, vec, v);
-  // n and `per` are multiples of 4, so the lanes of a block are all in or all out of range
-  MxOut q = o;
-  if (t >= n) q.pitch = 0;
-  mx_emit<BITS>(q, row, j, v);
+// Row and place of the t-th of a matrix's 8-value parts, `per` a row; 32-bit division where it does.
+DEV void mx_place(int64_t t, int64_t n, int per, int64_t& row, int& j) {
+  if (n <= 0x7fffffff) {
+    const uint32_t r = (uint32_t)t / (uint32_t)per;
+    row = r;
+    j = (int)((uint32_t)t - r * (uint32_t)per);
+  } else {
+    row = t / per;
+    j = (int)(t - row * per);
+  }
 }
 
-// one thread per 8 values
+// MX_EACH parts of 8 values a thread, a block's width apart; all loads first.  Bound by memory: per value
+// it reads the input once and writes bits / 8 + 1/32 bytes (and 2 with `values`).
+#define MX_EACH 4
+template <int TYPE, int BITS, bool VEC>
+__global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::T* x, int64_t ldx, int64_t n, MxOut o) {
+  const int per = o.pitch * 4;   // parts a row
+  const int64_t t0 = (int64_t)blockIdx.x * (256 * MX_EACH) + threadIdx.x;
+  Raw8<TYPE> raw[MX_EACH];
+  int64_t row;
+  int j;
+  mx_place(t0, n, per, row, j);
+  int64_t r = row;
+  int c = j;
+#pragma unroll
+  for (int i = 0; i < MX_EACH; ++i) {
+    const bool live = t0 + i * 256 < n;
+    raw[i].template load<VEC>(live ? x + r * ldx + 8 * c : x, live ? o.dim - 8 * c : 0);
+    for (c += 256; c >= per; c -= per) ++r;
+  }
+#pragma unroll
+  for (int i = 0; i < MX_EACH; ++i) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = raw[i].get(e);
+    // n and `per` are multiples of 4, so the lanes of a block of 32 are all in or all out of range
+    mx_emit<BITS>(o, row, t0 + i * 256 < n ? j : o.pitch * 4, v);
+    for (j += 256; j >= per; j -= per) ++row;
+  }
+}
+
+// MX_EACH parts of 8 values a thread
 template <int TYPE, int BITS>
 __global__ void __launch_bounds__(256) k_mx_values(MxOut o, int64_t n, typename Elem<TYPE>::T* out, int64_t ld, bool vec) {
   const int per = o.kb * 4;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= n) return;
-  const int64_t row = t / per;
-  const int j = (int)(t - row * per);
-  const uint8_t* d = o.codes + (row * per + j) * BITS;
-  uint32_t c[2];
-  c[0] = *(const uint32_t*)d;
-  c[1] = BITS == 8 ? ((const uint32_t*)d)[1] : 0u;
-  const uint32_t s = o.scales[row * o.pitch + (j >> 2)];
-  float u[8];
-  mx_decode<BITS>(c, u);
-  const float two = s == 255u ? __int_as_float(0x7fc00000) : mx_two((int)s - 127);
+  const int64_t t0 = (int64_t)blockIdx.x * (256 * MX_EACH) + threadIdx.x;
+  int64_t row;
+  int j;
+  mx_place(t0, n, per, row, j);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] *= two;
-  store8<TYPE>(out + row * ld + 8 * j, o.dim - 8 * j, vec, u);
+  for (int i = 0; i < MX_EACH; ++i) {
+    if (t0 + i * 256 >= n) return;
+    const uint8_t* d = o.codes + (row * per + j) * BITS;
+    uint32_t c[2];
+    c[0] = __ldg((const uint32_t*)d);
+    c[1] = BITS == 8 ? __ldg((const uint32_t*)d + 1) : 0u;
+    const uint32_t s = o.scales[row * o.pitch + (j >> 2)];
+    float u[8];
+    mx_decode<BITS>(c, u);
+    const float two = s == 255u ? __int_as_float(0x7fc00000) : mx_two((int)s - 127);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] *= two;
+    store8<TYPE>(out + row * ld + 8 * j, o.dim - 8 * j, vec, u);
+    for (j += 256; j >= per; j -= per) ++row;
+  }
 }

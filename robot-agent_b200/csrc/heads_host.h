@@ -49,3 +49,10 @@ static inline int mx_args(const char* who, int rows, int k, int bits, const uint
   if (!on16(codes) || !on16(scales)) return fail(SMG_ERR_ARGS, "%s: codes and scales must start on 16 bytes", who);
   return SMG_OK;
 }
+
+static inline MxDiv mx_div(int per) {
+  int shift = 0;
+  while ((1ll << shift) < per) ++shift;
+  const MxDiv d = {(uint32_t)per, (uint32_t)(((1ull << (31 + shift)) + (uint32_t)per - 1) / (uint32_t)per), shift};
+  return d;
+}

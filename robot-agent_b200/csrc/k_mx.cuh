@@ -4,9 +4,8 @@
 // Block rule: with m the largest magnitude, e = floor(log2 m) - emax (emax = 2 for e2m1, whose
 // largest value is 1.5 * 2^2; 8 for e4m3, 1.75 * 2^8), clamped to -127..127; the codes are the
 // nearest values of the format to x / 2^e, ties to even, saturating.  floor(log2 m) is m's exponent
-// field; m itself is taken as the largest magnitude BIT pattern, an unsigned maximum, under which
-// an infinity is above every number and a NaN above an infinity, so that such a block is seen and
-// gets the scale NaN (255) whatever its other values are.  x / 2^e is an exact product (2^-e is
+// field; m is taken with the maximum that hands NaN on, so that a block with an infinity or NaN is seen
+// and gets the scale NaN (255) whatever its other values are.  x / 2^e is an exact product (2^-e is
 // a normal float for every e that a block can have), so the only rounding is the conversion's.
 #pragma once
 #include <cuda_bf16.h>
@@ -42,31 +41,14 @@ struct Elem<SMG_EMB_F16> {
   static DEV __half down(float v) { return __float2half_rn(v); }
 };
 
-// p: the first of 8 values, of which n (<= 8, may be <= 0) exist; vec: p is 16-byte aligned
-template <int TYPE>
-DEV void load8(const typename Elem<TYPE>::T* p, int n, bool vec, float (&v)[8]) {
-  typedef typename Elem<TYPE>::T T;
-  if (vec && n >= 8) {
-    union { uint4 q[sizeof(T) / 2]; T t[8]; } u;
-    const uint4* s = (const uint4*)p;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.q[i] = __ldg(s + i);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = Elem<TYPE>::up(u.t[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? Elem<TYPE>::up(p[i]) : 0.f;
-  }
-}
-
-// The same in two steps, for kernels that first issue all of a row's loads: 8 values as they lie in
-// memory (none past n: zero bits are the value 0), and the floats they are.  VEC: p on 16 bytes, n a multiple of 8.
+// 8 values of a row as they lie in memory (zeros past n, which may be <= 0), and the floats they are: in two
+// steps, so that a kernel can issue all of its loads first.  VEC: p on 16 bytes, n a multiple of 8.
 template <int TYPE>
 struct Raw8 {
   typedef typename Elem<TYPE>::T T;
   union { uint4 q[sizeof(T) / 2]; T t[8]; };
   template <bool VEC>
-  DEV void load(const T* p, int n) {
+  DEV void load(const T* p, int n) {   // p is used only where n > 0
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = n > 0 ? __ldg((const uint4*)p + i) : make_uint4(0, 0, 0, 0);
@@ -97,11 +79,18 @@ DEV void store8(typename Elem<TYPE>::T* p, int n, bool vec, const float (&v)[8])
 // 2^e, -127 <= e <= 127
 DEV float mx_two(int e) { return __int_as_float(e > -127 ? (e + 127) << 23 : 1 << 22); }
 
-// scale byte of a block whose largest magnitude has the bit pattern m
+DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// scale byte of a block whose largest magnitude is m
 template <int BITS>
-DEV uint32_t mx_scale(uint32_t m) {
-  if (m >= 0x7f800000u) return 255u;
-  const int s = (int)(m >> 23) - (BITS == 4 ? 2 : 8);
+DEV uint32_t mx_scale(float m) {
+  const uint32_t b = __float_as_uint(m);
+  if (b >= 0x7f800000u) return 255u;
+  const int s = (int)(b >> 23) - (BITS == 4 ? 2 : 8);
   return (uint32_t)(s < 0 ? 0 : s);
 }
 
@@ -132,17 +121,39 @@ DEV void mx_codes(const float (&u)[8], uint32_t (&c)[2]) {
   }
 }
 
-// Codes of 8 values back to floats (without the scale).  An e2m1 code's 3 magnitude bits, put at the
-// border of a float's exponent and mantissa, are the value times 2^-126 (subnormal ones too).
-template <int BITS>
-DEV void mx_decode(const uint32_t (&c)[2], float (&u)[8]) {
-  if constexpr (BITS == 4) {
+// Codes of 8 e2m1 values to 8 bf16 ones (without the scale) times 2^-126: a code's 3 magnitude bits,
+// put at the border of exponent and mantissa, are that (subnormal ones too).
+DEV void mx_e2m1_bf16(uint32_t c, uint32_t (&p)[4]) {
+  const uint32_t lo = c & 0x0f0f0f0fu, hi = c >> 4 & 0x0f0f0f0fu;   // even and odd values, a byte each
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t n = c[0] >> (4 * i);
-      u[i] = __uint_as_float((n & 7u) << 22 | (n & 8u) << 28) * __uint_as_float(253u << 23);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w;   // value 2i in the low half, 2i + 1 in the high one
+    if (i == 0) w = __byte_perm(lo, hi, 0x7470) & 0x000f000fu;
+    else if (i == 1) w = __byte_perm(lo, hi, 0x7571) & 0x000f000fu;
+    else if (i == 2) w = __byte_perm(lo, hi, 0x7672) & 0x000f000fu;
+    else w = __byte_perm(lo, hi, 0x7773) & 0x000f000fu;
+    p[i] = (w << 6 & 0x01c001c0u) | (w << 12 & 0x80008000u);
+  }
+}
+
+DEV __nv_bfloat162 bf162(uint32_t bits) { return *(const __nv_bfloat162*)&bits; }
+DEV __nv_bfloat162 bf162_all(uint32_t one) { return bf162(one | one << 16); }
+
+// Codes of 8 values to the bf16 values they stand for, with the block's scale byte.  Products of
+// powers of two and values of 4 bits or fewer of mantissa: exact, but below 2^-126.
+template <int BITS>
+DEV void mx_values8(const uint32_t (&c)[2], uint32_t scale, uint32_t (&out)[4]) {
+  // 2^(scale - 127) in bf16 (subnormal for 0), or NaN
+  const uint32_t two = scale == 255u ? 0x7fc0u : scale ? scale << 7 : 0x40u;
+  if constexpr (BITS == 4) {
+    mx_e2m1_bf16(c[0], out);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 v = __hmul2(__hmul2(bf162(out[i]), bf162_all(253u << 7)), bf162_all(two));
+      out[i] = *(const uint32_t*)&v;
     }
   } else {
+    const float f = __uint_as_float(two << 16);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       uint32_t h[2];
@@ -155,12 +166,19 @@ DEV void mx_decode(const uint32_t (&c)[2], float (&u)[8]) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const __half2 p = *(const __half2*)&h[i];
-        u[4 * q + 2 * i] = __low2float(p);
-        u[4 * q + 2 * i + 1] = __high2float(p);
+        const __nv_bfloat162 v = __floats2bfloat162_rn(__low2float(p) * f, __high2float(p) * f);
+        out[2 * q + i] = *(const uint32_t*)&v;
       }
     }
   }
 }
+
+// Division of a place below 2^31 by `per`: (t * mul) >> (31 + shift), mul = ceil(2^(31 + shift) / per),
+// shift = ceil(log2 per)
+struct MxDiv {
+  uint32_t per, mul;
+  int shift;
+};
 
 struct MxOut {
   uint8_t* codes;      // rows of kb * 32 * bits / 8 bytes
@@ -173,17 +191,17 @@ struct MxOut {
 // hold one block and all 32 lanes of the warp call this together.  v is zero past dim.
 template <int BITS>
 DEV void mx_emit(const MxOut& o, int64_t row, int j, const float (&v)[8]) {
-  uint32_t m = 0;
+  float m = fabsf(v[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const int b = j >> 2;
   if (b >= o.pitch) return;
   const uint32_t s = mx_scale<BITS>(m);
   if (o.scales && !(j & 3)) o.scales[row * o.pitch + b] = (uint8_t)(b < o.kb ? s : 0u);
   if (b >= o.kb) return;
-  const float inv = mx_two(s == 255u ? 0 : 127 - (int)s);
+  const float inv = __uint_as_float(s == 255u ? 0x3f800000u : (254u - s) << 23);
   float u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) u[i] = v[i] * inv;
@@ -195,23 +213,29 @@ DEV void mx_emit(const MxOut& o, int64_t row, int j, const float (&v)[8]) {
     else *(uint2*)d = make_uint2(c[0], c[1]);
   }
   if (o.values) {
-    mx_decode<BITS>(c, u);
-    const float two = s == 255u ? __int_as_float(0x7fc00000) : mx_two((int)s - 127);
+    union { uint32_t w[4]; uint16_t h[8]; } q;
+    mx_values8<BITS>(c, s, q.w);
+    __nv_bfloat16* d = o.values + row * o.dim + 8 * j;
+    const int n = o.dim - 8 * j;
+    if (!(o.dim & 7)) {
+      if (n > 0) *(uint4*)d = make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] *= two;
-    store8<SMG_EMB_BF16>(o.values + row * o.dim + 8 * j, o.dim - 8 * j, !(o.dim & 7), u);
+      for (int i = 0; i < 8; ++i)
+        if (i < n) ((uint16_t*)d)[i] = q.h[i];
+    }
   }
 }
 
-// Row and place of the t-th of a matrix's 8-value parts, `per` a row; 32-bit division where it does.
-DEV void mx_place(int64_t t, int64_t n, int per, int64_t& row, int& j) {
+// Row and place of the t-th of a matrix's n 8-value parts
+DEV void mx_place(int64_t t, int64_t n, const MxDiv& d, int64_t& row, int& j) {
   if (n <= 0x7fffffff) {
-    const uint32_t r = (uint32_t)t / (uint32_t)per;
+    const uint32_t r = (uint32_t)((uint64_t)(uint32_t)t * d.mul >> (31 + d.shift));
     row = r;
-    j = (int)((uint32_t)t - r * (uint32_t)per);
+    j = (int)((uint32_t)t - r * d.per);
   } else {
-    row = t / per;
-    j = (int)(t - row * per);
+    row = t / d.per;
+    j = (int)(t - row * d.per);
   }
 }
 
@@ -219,54 +243,59 @@ DEV void mx_place(int64_t t, int64_t n, int per, int64_t& row, int& j) {
 // it reads the input once and writes bits / 8 + 1/32 bytes (and 2 with `values`).
 #define MX_EACH 4
 template <int TYPE, int BITS, bool VEC>
-__global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::T* x, int64_t ldx, int64_t n, MxOut o) {
-  const int per = o.pitch * 4;   // parts a row
+__global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::T* x, int64_t ldx, int64_t n, MxDiv div, MxOut o) {
   const int64_t t0 = (int64_t)blockIdx.x * (256 * MX_EACH) + threadIdx.x;
   Raw8<TYPE> raw[MX_EACH];
-  int64_t row;
-  int j;
-  mx_place(t0, n, per, row, j);
-  int64_t r = row;
-  int c = j;
+  int64_t row[MX_EACH];
+  int j[MX_EACH];
 #pragma unroll
   for (int i = 0; i < MX_EACH; ++i) {
-    const bool live = t0 + i * 256 < n;
-    raw[i].template load<VEC>(live ? x + r * ldx + 8 * c : x, live ? o.dim - 8 * c : 0);
-    for (c += 256; c >= per; c -= per) ++r;
+    mx_place(t0 + i * 256, n, div, row[i], j[i]);
+    // n and a row's parts are multiples of 4, so the lanes of a block of 32 are all in or all out of range
+    if (t0 + i * 256 >= n) { row[i] = 0; j[i] = o.pitch * 4; }
+    raw[i].template load<VEC>(x + row[i] * ldx + 8 * j[i], o.dim - 8 * j[i]);
   }
 #pragma unroll
   for (int i = 0; i < MX_EACH; ++i) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = raw[i].get(e);
-    // n and `per` are multiples of 4, so the lanes of a block of 32 are all in or all out of range
-    mx_emit<BITS>(o, row, t0 + i * 256 < n ? j : o.pitch * 4, v);
-    for (j += 256; j >= per; j -= per) ++row;
+    mx_emit<BITS>(o, row[i], j[i], v);
   }
 }
 
 // MX_EACH parts of 8 values a thread
 template <int TYPE, int BITS>
-__global__ void __launch_bounds__(256) k_mx_values(MxOut o, int64_t n, typename Elem<TYPE>::T* out, int64_t ld, bool vec) {
-  const int per = o.kb * 4;
+__global__ void __launch_bounds__(256) k_mx_values(MxOut o, int64_t n, MxDiv div, typename Elem<TYPE>::T* out, int64_t ld, bool vec) {
   const int64_t t0 = (int64_t)blockIdx.x * (256 * MX_EACH) + threadIdx.x;
-  int64_t row;
-  int j;
-  mx_place(t0, n, per, row, j);
 #pragma unroll
   for (int i = 0; i < MX_EACH; ++i) {
     if (t0 + i * 256 >= n) return;
-    const uint8_t* d = o.codes + (row * per + j) * BITS;
-    uint32_t c[2];
+    int64_t row;
+    int j;
+    mx_place(t0 + i * 256, n, div, row, j);
+    const uint8_t* d = o.codes + (row * o.kb * 4 + j) * BITS;
+    uint32_t c[2], q[4];
     c[0] = __ldg((const uint32_t*)d);
     c[1] = BITS == 8 ? __ldg((const uint32_t*)d + 1) : 0u;
     const uint32_t s = o.scales[row * o.pitch + (j >> 2)];
     float u[8];
-    mx_decode<BITS>(c, u);
-    const float two = s == 255u ? __int_as_float(0x7fc00000) : mx_two((int)s - 127);
+    if (TYPE == SMG_EMB_BF16) {
+      mx_values8<BITS>(c, s, q);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] *= two;
+      for (int e = 0; e < 4; ++e) {
+        u[2 * e] = __uint_as_float(q[e] << 16);
+        u[2 * e + 1] = __uint_as_float(q[e] & 0xffff0000u);
+      }
+    } else {   // the values without the scale are exact in bf16; the scale is applied in 32 bits
+      mx_values8<BITS>(c, 127, q);
+      const float two = s == 255u ? __int_as_float(0x7fc00000) : mx_two((int)s - 127);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        u[2 * e] = __uint_as_float(q[e] << 16) * two;
+        u[2 * e + 1] = __uint_as_float(q[e] & 0xffff0000u) * two;
+      }
+    }
     store8<TYPE>(out + row * ld + 8 * j, o.dim - 8 * j, vec, u);
-    for (j += 256; j >= per; j -= per) ++row;
   }
 }

@@ -35,10 +35,10 @@ int smg_mx_quantise(const void* x, int64_t ldx, int rows, int k, int type, int b
   if (int r = mx_blocks(who, n, &grid)) return r;
 #define CALL(TY)                                                                                                              \
   const Elem<TY>::T* p = (const Elem<TY>::T*)x;                                                                               \
-  if (vec && bits == 4) k_mx_quantise<TY, 4, true><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, o);                      \
-  else if (vec) k_mx_quantise<TY, 8, true><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, o);                              \
-  else if (bits == 4) k_mx_quantise<TY, 4, false><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, o);                       \
-  else k_mx_quantise<TY, 8, false><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, o)
+  if (vec && bits == 4) k_mx_quantise<TY, 4, true><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, mx_div(o.pitch * 4), o);                      \
+  else if (vec) k_mx_quantise<TY, 8, true><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, mx_div(o.pitch * 4), o);                              \
+  else if (bits == 4) k_mx_quantise<TY, 4, false><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, mx_div(o.pitch * 4), o);                       \
+  else k_mx_quantise<TY, 8, false><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, mx_div(o.pitch * 4), o)
   BY_TYPE(type, CALL);
 #undef CALL
   return launched(who);
@@ -58,8 +58,8 @@ int smg_mx_values(const uint8_t* codes, const uint8_t* scales, int rows, int k, 
   unsigned grid;
   if (int r = mx_blocks(who, n, &grid)) return r;
 #define CALL(TY)                                                                                                  \
-  if (bits == 4) k_mx_values<TY, 4><<<grid, 256, 0, (cudaStream_t)stream>>>(o, n, (Elem<TY>::T*)out, ld, vec);      \
-  else k_mx_values<TY, 8><<<grid, 256, 0, (cudaStream_t)stream>>>(o, n, (Elem<TY>::T*)out, ld, vec)
+  if (bits == 4) k_mx_values<TY, 4><<<grid, 256, 0, (cudaStream_t)stream>>>(o, n, mx_div(o.kb * 4), (Elem<TY>::T*)out, ld, vec);      \
+  else k_mx_values<TY, 8><<<grid, 256, 0, (cudaStream_t)stream>>>(o, n, mx_div(o.kb * 4), (Elem<TY>::T*)out, ld, vec)
   BY_TYPE(out_type, CALL);
 #undef CALL
   return launched(who);

@@ -29,11 +29,12 @@ static int operand(const char* who, const char* name, const void* p, int64_t ld,
   return SMG_OK;
 }
 
-// SMs of the current device
-static int sm_count() {
+// SMs of the current device, and which it is; 0 without one
+static int sm_count(int* device) {
   static std::atomic<int> known[64];
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  *device = dev;
   if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
   if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
@@ -92,9 +93,15 @@ static int launch(const char* who, const Operands& o, ProdArgs g, int type, cuda
   g.idesc = fmt << 7 | fmt << 10 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(PR_BM >> 4) << 24 | (KIND == 16 ? 1u << 4 : 1u << 23) |
             (FORM == FORM_DW ? 1u << 15 : 0u) | (FORM == FORM_DX || FORM == FORM_DW ? 1u << 16 : 0u);
   g.y_vec = rows16(g.y, g.ldy, g.y_type) && (FORM != FORM_DW || g.y_stride * size_of(g.y_type) % 16 == 0);
-  const int sms = sm_count();
-  const cudaError_t e = cudaFuncSetAttribute(k_prod<KIND, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-  if (!sms || e != cudaSuccess) return fail(SMG_ERR_DEVICE, "%s: no usable device (%s)", who, cudaGetErrorString(cudaGetLastError()));
+  static std::atomic<uint64_t> ready;   // devices on which this kernel has its shared memory
+  int dev = 0;
+  const int sms = sm_count(&dev);
+  if (!sms) return fail(SMG_ERR_DEVICE, "%s: no usable device (%s)", who, cudaGetErrorString(cudaGetLastError()));
+  if (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(k_prod<KIND, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return fail(SMG_ERR_DEVICE, "%s: %s", who, cudaGetErrorString(e));
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   k_prod<KIND, BN, FORM><<<(unsigned)std::min<int64_t>(sms, row_tiles * per), PR_THREADS, S::SMEM, st>>>(tA, tB, g);
   return launched(who);
 }

@@ -22,10 +22,11 @@
 //   warp 0      TMA loads of P and Q into the ring (full / empty barriers);
 //   warp 1      one thread issues the MMAs; tfull[a] when a tile's are done, tempty[a] before an
 //               accumulator's reuse;
-//   warps 2, 3  what the loads leave to be done, reported on fixed[s]: microscaled rows: the scales, 4 bytes
-//               of a row at a time, into the order that the tensor memory wants (row r of 128 at 16 (r % 32)
-//               + 4 (r / 32)); DW: zeros over the rows past the group's end in its last block, where the load brought the
-//               next group's rows (both operands, since a NaN times zero is none);
+//   warps 2, 3  what the loads leave to be done.  Microscaled rows: the scales, in a ring of their own
+//               (cfull / cempty), 16 bytes of a row at a time, put into the order that the tensor memory
+//               wants (row r of 128 at 16 (r % 32) + 4 (r / 32) of 512 bytes for each 4 blocks).  DW: zeros over the
+//               rows past the group's end in its last block, where the load brought the next group's
+//               rows (in both operands, since zero times NaN is NaN), reported on fixed[s];
 //   warps 4-11  read D from tensor memory, round once and store.  Rows past the group's end and
 //               columns past the width are computed and not stored.
 // Every wait is bounded, or goes on only until another role's bounded wait has run out; then the
@@ -63,15 +64,15 @@ struct ProdArgs {
 template <int KIND, int BN>
 struct ProdShape {
   static constexpr int QCH = (BN + 127) / 128;                          // 128-row parts of Q
-  static constexpr int SFW = KIND == 16 ? 0 : KIND == 8 ? 1 : 2;        // 4-byte scale words of a row and block
-  static constexpr int P_BYTES = PR_BM * 128, Q_BYTES = BN * 128, S_BYTES = (1 + QCH) * SFW * 512;
-  static constexpr int STAGE = P_BYTES + Q_BYTES + S_BYTES;
-  static constexpr int ROOM = PR_SMEM_MAX - 1024 - PR_STAGING - PR_GROUP_BYTES - 512;
-  static constexpr int STAGES = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
-  static constexpr int SMEM = STAGES * STAGE + 1024 + PR_STAGING + PR_GROUP_BYTES + 512;
-  static constexpr int SFC = (1 + QCH) * SFW * 4;                       // tensor-memory columns of a stage's scales
-  static constexpr int COLS = 2 * BN + STAGES * SFC;
-  static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static constexpr int P_BYTES = PR_BM * 128, Q_BYTES = BN * 128, STAGE = P_BYTES + Q_BYTES;
+  // scales come in chunks of 4 words of 4 bytes a row (512 values): 2 (e2m1) or 4 (e4m3) stages
+  static constexpr int CHUNK = KIND == 16 ? 0 : (1 + QCH) * 4 * 512, CHUNKS = 3, CHUNK_STAGES = KIND == 4 ? 2 : 4;
+  static constexpr int SFC = KIND == 16 ? 0 : (1 + QCH) * 16;           // and their tensor-memory columns, two chunks in turn
+  static constexpr int FIXED = CHUNKS * CHUNK + 1024 + PR_STAGING + PR_GROUP_BYTES + 512;
+  static constexpr int STAGES = (PR_SMEM_MAX - FIXED) / STAGE > 8 ? 8 : (PR_SMEM_MAX - FIXED) / STAGE;
+  static constexpr int SMEM = STAGES * STAGE + FIXED;
+  static constexpr int COLS = 2 * BN + 2 * SFC;
+  static constexpr int TMEM = 512;   // all of it: its first column is then 0, a constant in every address below
   static_assert(COLS <= 512 && STAGES >= 3, "tile too large");
 };
 
@@ -123,6 +124,13 @@ DEV void pr_mma_mx(uint32_t d, uint64_t p, uint64_t q, uint32_t idesc, uint32_t 
 
 DEV void pr_copy_scales(uint32_t tmem, const void* p) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(pr_desc_scales(p)) : "memory");
+}
+
+// true in one lane of a converged warp
+DEV bool pr_elect() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 DEV void pr_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -179,27 +187,35 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   unsigned char* sP = base;
   unsigned char* sQ = sP + STAGES * S::P_BYTES;
   unsigned char* sS = sQ + STAGES * S::Q_BYTES;
-  unsigned char* staging = sS + STAGES * S::S_BYTES;
+  unsigned char* staging = sS + S::CHUNKS * S::CHUNK;
   int* s_beg = (int*)(staging + PR_STAGING);
   int* s_end = s_beg + SMG_PROD_MAX_GROUPS;
   int* s_cum = s_end + SMG_PROD_MAX_GROUPS;
   uint64_t* full = (uint64_t*)(((uintptr_t)(s_cum + SMG_PROD_MAX_GROUPS + 1) + 7) & ~(uintptr_t)7);
   uint64_t* empty = full + STAGES;
   uint64_t* fixed = empty + STAGES;
-  uint64_t* tfull = fixed + STAGES;
+  uint64_t* cfull = fixed + STAGES;      // microscaled rows: a chunk of scales has landed,
+  uint64_t* cempty = cfull + S::CHUNKS;  // has been copied to tensor memory,
+  uint64_t* cdone = cempty + S::CHUNKS;  // and the MMAs that use the copy are done
+  uint64_t* tfull = cdone + 2;
   uint64_t* tempty = tfull + 2;
   uint64_t* done = tempty + 2;
   uint32_t* tmem_slot = (uint32_t*)(done + 1);
   __shared__ int sh_fail;
   volatile int* failed = &sh_fail;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
       ag_mbar_init(&full[s], 1);
       ag_mbar_init(&empty[s], 1);
-      ag_mbar_init(&fixed[s], KIND == 16 ? PR_HELPERS / 32 : PR_HELPERS);
+      ag_mbar_init(&fixed[s], PR_HELPERS / 32);
     }
+    for (int s = 0; s < S::CHUNKS; ++s) {
+      ag_mbar_init(&cfull[s], PR_HELPERS);
+      ag_mbar_init(&cempty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) ag_mbar_init(&cdone[a], 1);
     for (int a = 0; a < 2; ++a) {
       ag_mbar_init(&tfull[a], 1);
       ag_mbar_init(&tempty[a], PR_EPI_WARPS);
@@ -233,7 +249,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     for (int i = tid; i < g.n_groups; i += PR_THREADS) s_beg[i] = s_end[i] = 0;
     __syncthreads();
   }
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;
+  if (tid == 0 && *tmem_slot != tmem) *failed = 1;
   constexpr int RT = FORM == FORM_YT ? BN : PR_BM;
   if (warp == 0) {   // first row tile of every group
     int at = 0;
@@ -256,94 +273,106 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   T.beg = s_beg; T.end = s_end; T.cum = s_cum;
   T.n_groups = g.n_groups;
   T.fixed = FORM == FORM_DW ? g.p_tiles * g.q_tiles : FORM == FORM_YT ? g.p_tiles : g.q_tiles;
-  T.total = s_cum[g.n_groups] * T.fixed;
+  T.total = *failed ? 0 : s_cum[g.n_groups] * T.fixed;
   const int red = FORM == FORM_DX ? g.n : g.k;   // (DW: the group's rows)
   bool ok = true;
 
-  if (warp == 0) {
-    if (lane == 0) {   // loads
-      uint32_t it = 0;
-      for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x) {
-        const ProdTile c = prod_tile<FORM, BN>(T, t);
-        const int nk = ((FORM == FORM_DW ? c.r1 - c.r0 : red) + BK - 1) / BK;
-        for (int kb = 0; kb < nk; ++kb, ++it) {
-          const int s = (int)(it % STAGES);
-          if (it >= STAGES && !ag_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
-          unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
-          ag_expect_tx(&full[s], S::P_BYTES + S::Q_BYTES);
-          const int x = KIND == 16 ? kb * BK : kb * 128;   // microscaled rows are loaded as bytes
-          if (FORM == FORM_Y) {
-            ag_tma_2d(&tmA, &full[s], p, x, c.r0);
-            pr_tma_3d(&tmB, &full[s], q, x, c.f * BN, c.g);
-          } else if (FORM == FORM_YT) {
-            pr_tma_3d(&tmB, &full[s], p, x, c.f * PR_BM, c.g);
-            ag_tma_2d(&tmA, &full[s], q, x, c.r0);
-          } else if (FORM == FORM_DX) {
-            ag_tma_2d(&tmA, &full[s], p, x, c.r0);
+  // The loads and the MMAs are issued by one elected lane, in code that the whole warp runs: their
+  // operands live in uniform registers, and from a single thread's own code each MMA took 115 cycles to
+  // issue, whatever its width (measured; 32 to 128 run so).
+  if (warp == 0) {   // loads
+    const bool one = pr_elect();
+    uint32_t it = 0;
+    for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x) {
+      const ProdTile c = prod_tile<FORM, BN>(T, t);
+      const int nk = ((FORM == FORM_DW ? c.r1 - c.r0 : red) + BK - 1) / BK;
+      for (int kb = 0; kb < nk; ++kb, ++it) {
+        const int s = (int)(it % STAGES);
+        if (it >= STAGES && !ag_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
+        unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
+        if (!one) continue;
+        ag_expect_tx(&full[s], S::P_BYTES + S::Q_BYTES);
+        const int x = KIND == 16 ? kb * BK : kb * 128;   // microscaled rows are loaded as bytes
+        if (FORM == FORM_Y) {
+          ag_tma_2d(&tmA, &full[s], p, x, c.r0);
+          pr_tma_3d(&tmB, &full[s], q, x, c.f * BN, c.g);
+        } else if (FORM == FORM_YT) {
+          pr_tma_3d(&tmB, &full[s], p, x, c.f * PR_BM, c.g);
+          ag_tma_2d(&tmA, &full[s], q, x, c.r0);
+        } else if (FORM == FORM_DX) {
+          ag_tma_2d(&tmA, &full[s], p, x, c.r0);
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j) pr_tma_3d(&tmB, &full[s], q + j * 8192, c.f * BN + j * 64, x, c.g);
-          } else {
-            const int m0 = c.f % g.p_tiles * PR_BM, n0 = c.f / g.p_tiles * BN;
+          for (int j = 0; j < BN / 64; ++j) pr_tma_3d(&tmB, &full[s], q + j * 8192, c.f * BN + j * 64, x, c.g);
+        } else {
+          const int m0 = c.f % g.p_tiles * PR_BM, n0 = c.f / g.p_tiles * BN;
 #pragma unroll
-            for (int j = 0; j < PR_BM / 64; ++j) ag_tma_2d(&tmA, &full[s], p + j * 8192, m0 + j * 64, c.r0 + x);
+          for (int j = 0; j < PR_BM / 64; ++j) ag_tma_2d(&tmA, &full[s], p + j * 8192, m0 + j * 64, c.r0 + x);
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j) ag_tma_2d(&tmB, &full[s], q + j * 8192, n0 + j * 64, c.r0 + x);
-          }
+          for (int j = 0; j < BN / 64; ++j) ag_tma_2d(&tmB, &full[s], q + j * 8192, n0 + j * 64, c.r0 + x);
         }
       }
-      // the last loads must have landed before the CTA ends
-      const uint32_t first = it > STAGES ? it - STAGES : 0;
-      for (uint32_t j = first; j < it; ++j) ok = ag_wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
-      if (!ok) *failed = 1;
     }
-  } else if (warp == 1) {
-    if (lane == 0) {   // MMAs
-      uint32_t it = 0, j = 0;
-      for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x, ++j) {
-        const ProdTile c = prod_tile<FORM, BN>(T, t);
-        const int len = FORM == FORM_DW ? c.r1 - c.r0 : red, nk = (len + BK - 1) / BK;
-        const uint32_t acc = j & 1u;
-        if (j >= 2 && !ag_wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
+    // the last loads must have landed before the CTA ends
+    const uint32_t first = it > STAGES ? it - STAGES : 0;
+    for (uint32_t j = first; j < it; ++j) ok = ag_wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
+    if (!ok) *failed = 1;
+  } else if (warp == 1) {   // MMAs
+    const bool one = pr_elect();
+    uint32_t it = 0, j = 0, ci = 0;
+    for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x, ++j) {
+      const ProdTile c = prod_tile<FORM, BN>(T, t);
+      const int len = FORM == FORM_DW ? c.r1 - c.r0 : red, nk = (len + BK - 1) / BK;
+      const uint32_t acc = j & 1u;
+      if (j >= 2 && !ag_wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
+      ag_fence_after();
+      const uint32_t d = tmem + acc * BN;
+      for (int kb = 0; kb < nk; ++kb, ++it) {
+        const int s = (int)(it % STAGES);
+        const uint32_t ph = (it / STAGES) & 1u;
+        const int left = len - kb * BK;
+        if (!ag_wait(&full[s], ph)) { ok = false; break; }
+        if (FORM == FORM_DW && !ag_wait(&fixed[s], ph)) { ok = false; break; }
+        if (KIND != 16 && kb % S::CHUNK_STAGES == 0) {
+          if (ci >= 2 && !ag_wait(&cdone[ci & 1u], ((ci >> 1) & 1u) ^ 1u)) { ok = false; break; }
+          if (!ag_wait(&cfull[ci % S::CHUNKS], (ci / S::CHUNKS) & 1u)) { ok = false; break; }
+          pr_proxy_fence();   // the scales were written by ordinary copies
+        }
         ag_fence_after();
-        const uint32_t d = tmem + acc * BN;
-        for (int kb = 0; kb < nk; ++kb, ++it) {
-          const int s = (int)(it % STAGES);
-          const uint32_t ph = (it / STAGES) & 1u;
-          const int left = len - kb * BK;
-          if (!ag_wait(&full[s], ph)) { ok = false; break; }
-          if (HELP && !ag_wait(&fixed[s], ph)) { ok = false; break; }
-          if (KIND != 16) pr_proxy_fence();   // the scales were written by ordinary copies
-          ag_fence_after();
-          const unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
-          const uint64_t dp = P_MN ? pr_desc_mn(p) : ag_desc(p), dq = Q_MN ? pr_desc_mn(q) : ag_desc(q);
-          const int subs = left >= BK ? 4 : (left + SUB - 1) / SUB;
+        const unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
+        const uint64_t dp = P_MN ? pr_desc_mn(p) : ag_desc(p), dq = Q_MN ? pr_desc_mn(q) : ag_desc(q);
+        const int subs = left >= BK ? 4 : (left + SUB - 1) / SUB;
+        if (one) {
           if constexpr (KIND == 16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (i < subs) pr_mma16(d, dp + i * (P_MN ? 128 : 2), dq + i * (Q_MN ? 128 : 2), g.idesc, (kb | i) != 0);
           } else {
-            const unsigned char* sc = sS + s * S::S_BYTES;
-            const uint32_t tp = tmem + 2 * BN + s * S::SFC, tq = tp + S::SFW * 4;
+            const uint32_t tp = tmem + 2 * BN + (ci & 1u) * S::SFC, tq = tp + 16;
+            if (kb % S::CHUNK_STAGES == 0) {
+              const unsigned char* sc = sS + ci % S::CHUNKS * S::CHUNK;
 #pragma unroll
-            for (int i = 0; i < S::SFW; ++i) pr_copy_scales(tp + 4 * i, sc + 512 * i);
-#pragma unroll
-            for (int i = 0; i < S::SFW * S::QCH; ++i) pr_copy_scales(tq + 4 * i, sc + 512 * (S::SFW + i));
+              for (int i = 0; i < 4 * (1 + S::QCH); ++i) pr_copy_scales(tp + 4 * i, sc + 512 * i);
+              ag_commit(&cempty[ci % S::CHUNKS]);
+            }
+            const uint32_t w0 = KIND == 4 ? kb % 2 * 2 : kb % 4;   // the stage's first word of the chunk
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               if (i < subs) {
                 // an MMA's 2 scales of a row (e2m1) are half a word, its one (e4m3) is a byte of it
-                const uint32_t w = KIND == 4 ? i / 2 : 0, id = KIND == 4 ? (i & 1) * 2 : i;
+                const uint32_t w = w0 + (KIND == 4 ? i / 2 : 0), id = KIND == 4 ? (i & 1) * 2 : i;
                 pr_mma_mx<KIND>(d, dp + i * 2, dq + i * 2, g.idesc | id << 29 | id << 4, tp + 4 * w, tq + 4 * S::QCH * w, (kb | i) != 0);
               }
             }
+            if (kb % S::CHUNK_STAGES == S::CHUNK_STAGES - 1 || kb == nk - 1) ag_commit(&cdone[ci & 1u]);
           }
           ag_commit(&empty[s]);
         }
-        ag_commit(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
+        if (KIND != 16 && (kb % S::CHUNK_STAGES == S::CHUNK_STAGES - 1 || kb == nk - 1)) ++ci;
       }
-      ag_commit(done);   // every issued MMA has completed before the tensor memory is freed
-      if (!ag_wait(done, 0) || !ok) *failed = 1;
+      if (one) ag_commit(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
     }
+    if (one) ag_commit(done);   // every issued MMA has completed before the tensor memory is freed
+    if (!ag_wait(done, 0) || !ok) *failed = 1;
   } else if (warp < 4) {
     if (HELP) {
       const int h = tid - 64;
@@ -351,33 +380,32 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x) {
         const ProdTile c = prod_tile<FORM, BN>(T, t);
         if constexpr (KIND != 16) {
-          const int nk = (red + BK - 1) / BK;
           // rows of w_g and rows of x, whichever is P
           const int w0 = c.f * (FORM == FORM_YT ? PR_BM : BN);
           const int p_lim = FORM == FORM_YT ? g.n - w0 : c.r1 - c.r0, q_lim = FORM == FORM_YT ? c.r1 - c.r0 : g.n - w0;
           const int64_t wr = (int64_t)c.g * g.n + w0, xr = c.r0;
           const uint8_t* ps = (FORM == FORM_YT ? g.sb + wr * g.pitch : g.sa + xr * g.pitch);
           const uint8_t* qs = (FORM == FORM_YT ? g.sa + xr * g.pitch : g.sb + wr * g.pitch);
-          for (int kb = 0; kb < nk; ++kb, ++it) {
-            const int s = (int)(it % STAGES);
-            if (it >= STAGES && !ag_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
-            const uint32_t sc = ag_smem(sS + s * S::S_BYTES);
+          // 8 rows x 16 bytes a warp and step: thread h has word h % 4 of the rows h / 4, h / 4 + 16, ...
+          const int r0 = h >> 2, w = h & 3;
+          for (int k0 = 0; k0 < g.pitch; k0 += 16, ++it) {
+            const uint32_t s = it % S::CHUNKS;
+            if (it >= S::CHUNKS && !ag_wait(&cempty[s], ((it / S::CHUNKS) & 1u) ^ 1u)) { ok = false; break; }
+            const uint32_t sc = ag_smem(sS + s * S::CHUNK);
+            if (k0 + 4 * w < g.pitch) {
 #pragma unroll
-            for (int w = 0; w < S::SFW; ++w) {
-              const int col = (kb * S::SFW + w) * 4;
-#pragma unroll
-              for (int r0 = 0; r0 < PR_BM + BN; r0 += PR_HELPERS) {
-                const int rr = r0 + h, r = rr < PR_BM ? rr : rr - PR_BM;
-                if (rr >= PR_BM + BN) break;
-                const bool is_p = rr < PR_BM;
-                const bool live = col < g.pitch && r < (is_p ? p_lim : q_lim);
-                const uint8_t* src = live ? (is_p ? ps : qs) + (int64_t)r * g.pitch + col : g.sa;
-                const uint32_t part = is_p ? w : S::SFW + w * S::QCH + (r >> 7);
-                const uint32_t dst = sc + 512 * part + (r & 31) * 16 + ((r >> 5) & 3) * 4;
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+              for (int i = 0; i < (PR_BM + BN) / 16; ++i) {
+                const bool is_p = i < PR_BM / 16;
+                const int r = r0 + 16 * (is_p ? i : i - PR_BM / 16);
+                const uint32_t part = is_p ? w : 4 + w * S::QCH + (r >> 7);
+                // (the scales of rows that are not there are left as they are: they touch only what is not stored)
+                if (r < (is_p ? p_lim : q_lim))
+                  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 512 * part + (r & 31) * 16 + ((r >> 5) & 3) * 4),
+                               "l"((is_p ? ps : qs) + (int64_t)r * g.pitch + k0 + 4 * w)
+                               : "memory");
               }
             }
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ag_smem(&fixed[s])) : "memory");
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ag_smem(&cfull[s])) : "memory");
           }
         } else {
           const int len = c.r1 - c.r0;

@@ -27,8 +27,15 @@
 //               wants (row r of 128 at 16 (r % 32) + 4 (r / 32) of 512 bytes for each 4 blocks).  DW: zeros over the
 //               rows past the group's end in its last block, where the load brought the next group's
 //               rows (in both operands, since zero times NaN is NaN), reported on fixed[s];
+//               Pairs: they pass a landed stage on to the leader's fixed[s];
 //   warps 4-11  read D from tensor memory, round once and store.  Rows past the group's end and
 //               columns past the width are computed and not stored.
+// Pairs (PAIR): two CTAs of a cluster work on one tile of 256 rows of P.  Each loads its own 128 rows
+// of P and one half of Q and keeps the sums of its rows; rank 0 issues the MMAs of both, which read
+// each half of Q once for the two.  That is what the single form lacks: at 128 x 256 a CTA writes 48 KB into
+// shared memory and reads 48 KB out of it for 512 cycles of MMAs, 192 bytes a cycle where an SM has 128;
+// in a pair it is 32 + 32 KB.
+//
 // Every wait is bounded, or goes on only until another role's bounded wait has run out; then the
 // roles run out too, SMG_PROD_TIMEOUT is set, and the CTA waits (bounded) for its own copies and
 // MMAs before it frees the tensor memory.
@@ -61,10 +68,11 @@ struct ProdArgs {
 #define PR_GROUP_BYTES ((3 * SMG_PROD_MAX_GROUPS + 1) * 4)
 
 // KIND 16: f16 or bf16; 8, 4: microscaled
-template <int KIND, int BN>
+template <int KIND, int BN, bool PAIR>
 struct ProdShape {
+  static constexpr int QR = PAIR ? BN / 2 : BN;                         // rows of Q that a CTA holds
   static constexpr int QCH = (BN + 127) / 128;                          // 128-row parts of Q
-  static constexpr int P_BYTES = PR_BM * 128, Q_BYTES = BN * 128, STAGE = P_BYTES + Q_BYTES;
+  static constexpr int P_BYTES = PR_BM * 128, Q_BYTES = QR * 128, STAGE = P_BYTES + Q_BYTES;
   // scales come in chunks of 4 words of 4 bytes a row (512 values): 2 (e2m1) or 4 (e4m3) stages
   static constexpr int CHUNK = KIND == 16 ? 0 : (1 + QCH) * 4 * 512, CHUNKS = 3, CHUNK_STAGES = KIND == 4 ? 2 : 4;
   static constexpr int SFC = KIND == 16 ? 0 : (1 + QCH) * 16;           // and their tensor-memory columns, two chunks in turn
@@ -98,12 +106,20 @@ DEV uint64_t pr_desc_scales(const void* p) {
   return (uint64_t)((a >> 4) & 0x3fffu) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
 
+template <bool PAIR>
 DEV void pr_mma16(uint32_t d, uint64_t p, uint64_t q, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(p), "l"(q), "r"(idesc), "r"(accum));
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(p), "l"(q), "r"(idesc), "r"(accum));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(p), "l"(q), "r"(idesc), "r"(accum));
 }
 
 template <int KIND>
@@ -136,6 +152,47 @@ DEV bool pr_elect() {
 DEV void pr_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 DEV void pr_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ag_smem(b)) : "memory"); }
 
+// ---- the pair of CTAs (a cluster of 2): rank 0 issues the MMAs of both ----
+DEV uint32_t pr_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// Arrival on the leader's barrier that lies where b does here.  Without cluster-wide release and acquire:
+// what it reports is data of asynchronous copies that have landed (or a read that is over), and with
+// them on every stage the products ran at 0.4 of this speed.
+DEV void pr_arrive_leader(uint64_t* b) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(ag_smem(b))
+      : "memory");
+}
+
+// arrives on b here (PAIR: there and here) when the MMAs issued so far are done
+template <bool PAIR>
+DEV void pr_commit(uint64_t* b) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(ag_smem(b)),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else
+    ag_commit(b);
+}
+
+// the same after ordinary writes to shared memory that the leader's MMAs read
+DEV void pr_release_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+template <bool PAIR>
+DEV void pr_cluster_sync() {
+  if constexpr (PAIR)
+    asm volatile(
+        "barrier.cluster.arrive.release.aligned;\n\t"
+        "barrier.cluster.wait.acquire.aligned;" ::
+            : "memory");
+}
+
 // A wait that may rightly last as long as a whole tile: it goes on while no role has failed (their
 // own waits are bounded).
 DEV bool pr_wait_long(uint64_t* b, uint32_t parity, volatile int* failed) {
@@ -156,7 +213,7 @@ struct ProdTile {
   int f;                        // index along the fixed axes
 };
 
-template <int FORM, int BN>
+template <int FORM, int BN, bool PAIR>
 DEV ProdTile prod_tile(const ProdTiles& T, int t) {
   const int u = t / T.fixed;
   int lo = 0, hi = T.n_groups;  // the last group whose first row tile is <= u (empty groups have none)
@@ -168,20 +225,22 @@ DEV ProdTile prod_tile(const ProdTiles& T, int t) {
   ProdTile r;
   r.g = lo;
   r.f = t - u * T.fixed;
-  r.r0 = T.beg[lo] + (FORM == FORM_DW ? 0 : (u - T.cum[lo]) * (FORM == FORM_YT ? BN : PR_BM));
+  r.r0 = T.beg[lo] + (FORM == FORM_DW ? 0 : (u - T.cum[lo]) * (FORM == FORM_YT ? BN : PAIR ? 2 * PR_BM : PR_BM));
   r.r1 = T.end[lo];
   return r;
 }
 
-template <int KIND, int BN, int FORM>
+template <int KIND, int BN, int FORM, bool PAIR>
 __global__ void __launch_bounds__(PR_THREADS, 1)
     k_prod(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ ProdArgs g) {
-  using S = ProdShape<KIND, BN>;
+  using S = ProdShape<KIND, BN, PAIR>;
+  static_assert(!PAIR || (KIND == 16 && FORM != FORM_YT), "pairs: 16 bits, rows as P");
   constexpr int STAGES = S::STAGES;
   constexpr bool P_MN = FORM == FORM_DW, Q_MN = FORM == FORM_DX || FORM == FORM_DW;
   constexpr int BK = P_MN || Q_MN ? 64 : 1024 / KIND;   // values of the reduction axis in a stage
   constexpr int SUB = BK / 4;                           // and in an MMA
-  constexpr bool HELP = KIND != 16 || FORM == FORM_DW;
+  constexpr bool RELAY = PAIR || FORM == FORM_DW;       // warps 2, 3 pass every stage on
+  constexpr int RELAYS = FORM == FORM_DW ? PR_HELPERS / 32 : 1;
   extern __shared__ unsigned char pr_raw[];
   unsigned char* base = (unsigned char*)(((uintptr_t)pr_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* sP = base;
@@ -209,7 +268,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     for (int s = 0; s < STAGES; ++s) {
       ag_mbar_init(&full[s], 1);
       ag_mbar_init(&empty[s], 1);
-      ag_mbar_init(&fixed[s], PR_HELPERS / 32);
+      ag_mbar_init(&fixed[s], RELAYS * (PAIR ? 2 : 1));
     }
     for (int s = 0; s < S::CHUNKS; ++s) {
       ag_mbar_init(&cfull[s], PR_HELPERS);
@@ -218,16 +277,24 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     for (int a = 0; a < 2; ++a) ag_mbar_init(&cdone[a], 1);
     for (int a = 0; a < 2; ++a) {
       ag_mbar_init(&tfull[a], 1);
-      ag_mbar_init(&tempty[a], PR_EPI_WARPS);
+      ag_mbar_init(&tempty[a], PR_EPI_WARPS * (PAIR ? 2 : 1));
     }
     ag_mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh_fail = 0;
   }
+  __syncwarp();
+  pr_cluster_sync<PAIR>();   // the other's barriers exist
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ag_smem(tmem_slot)), "r"(S::TMEM)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ag_smem(tmem_slot)), "r"(S::TMEM)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ag_smem(tmem_slot)), "r"(S::TMEM)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   // groups: offsets that break the rules are reported, and every group is then taken as empty
   int bad = 0;
@@ -251,7 +318,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   }
   constexpr uint32_t tmem = 0;
   if (tid == 0 && *tmem_slot != tmem) *failed = 1;
-  constexpr int RT = FORM == FORM_YT ? BN : PR_BM;
+  constexpr int RT = FORM == FORM_YT ? BN : PAIR ? 2 * PR_BM : PR_BM;
+  // which of a pair's 128 rows of P (and of its halves of Q) are this CTA's; the pairs walk the tiles
+  const int rank = PAIR ? (int)pr_rank() : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
   if (warp == 0) {   // first row tile of every group
     int at = 0;
     for (int i0 = 0; i0 < g.n_groups; i0 += 32) {
@@ -283,8 +352,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   if (warp == 0) {   // loads
     const bool one = pr_elect();
     uint32_t it = 0;
-    for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x) {
-      const ProdTile c = prod_tile<FORM, BN>(T, t);
+    for (int t = first; t < T.total && ok; t += step) {
+      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
       const int nk = ((FORM == FORM_DW ? c.r1 - c.r0 : red) + BK - 1) / BK;
       for (int kb = 0; kb < nk; ++kb, ++it) {
         const int s = (int)(it % STAGES);
@@ -294,33 +363,32 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         ag_expect_tx(&full[s], S::P_BYTES + S::Q_BYTES);
         const int x = KIND == 16 ? kb * BK : kb * 128;   // microscaled rows are loaded as bytes
         if (FORM == FORM_Y) {
-          ag_tma_2d(&tmA, &full[s], p, x, c.r0);
-          pr_tma_3d(&tmB, &full[s], q, x, c.f * BN, c.g);
+          ag_tma_2d(&tmA, &full[s], p, x, c.r0 + rank * PR_BM);
+          pr_tma_3d(&tmB, &full[s], q, x, c.f * BN + rank * S::QR, c.g);
         } else if (FORM == FORM_YT) {
           pr_tma_3d(&tmB, &full[s], p, x, c.f * PR_BM, c.g);
           ag_tma_2d(&tmA, &full[s], q, x, c.r0);
         } else if (FORM == FORM_DX) {
-          ag_tma_2d(&tmA, &full[s], p, x, c.r0);
+          ag_tma_2d(&tmA, &full[s], p, x, c.r0 + rank * PR_BM);
 #pragma unroll
-          for (int j = 0; j < BN / 64; ++j) pr_tma_3d(&tmB, &full[s], q + j * 8192, c.f * BN + j * 64, x, c.g);
+          for (int j = 0; j < S::QR / 64; ++j) pr_tma_3d(&tmB, &full[s], q + j * 8192, c.f * BN + rank * S::QR + j * 64, x, c.g);
         } else {
-          const int m0 = c.f % g.p_tiles * PR_BM, n0 = c.f / g.p_tiles * BN;
+          const int m0 = c.f % g.p_tiles * RT + rank * PR_BM, n0 = c.f / g.p_tiles * BN + rank * S::QR;
 #pragma unroll
           for (int j = 0; j < PR_BM / 64; ++j) ag_tma_2d(&tmA, &full[s], p + j * 8192, m0 + j * 64, c.r0 + x);
 #pragma unroll
-          for (int j = 0; j < BN / 64; ++j) ag_tma_2d(&tmB, &full[s], q + j * 8192, n0 + j * 64, c.r0 + x);
+          for (int j = 0; j < S::QR / 64; ++j) ag_tma_2d(&tmB, &full[s], q + j * 8192, n0 + j * 64, c.r0 + x);
         }
       }
     }
     // the last loads must have landed before the CTA ends
-    const uint32_t first = it > STAGES ? it - STAGES : 0;
-    for (uint32_t j = first; j < it; ++j) ok = ag_wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
+    for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j) ok = ag_wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
     if (!ok) *failed = 1;
-  } else if (warp == 1) {   // MMAs
+  } else if (warp == 1 && rank == 0) {   // MMAs
     const bool one = pr_elect();
     uint32_t it = 0, j = 0, ci = 0;
-    for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x, ++j) {
-      const ProdTile c = prod_tile<FORM, BN>(T, t);
+    for (int t = first; t < T.total && ok; t += step, ++j) {
+      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
       const int len = FORM == FORM_DW ? c.r1 - c.r0 : red, nk = (len + BK - 1) / BK;
       const uint32_t acc = j & 1u;
       if (j >= 2 && !ag_wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
@@ -330,8 +398,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         const int s = (int)(it % STAGES);
         const uint32_t ph = (it / STAGES) & 1u;
         const int left = len - kb * BK;
-        if (!ag_wait(&full[s], ph)) { ok = false; break; }
-        if (FORM == FORM_DW && !ag_wait(&fixed[s], ph)) { ok = false; break; }
+        if (!ag_wait(RELAY ? &fixed[s] : &full[s], ph)) { ok = false; break; }
         if (KIND != 16 && kb % S::CHUNK_STAGES == 0) {
           if (ci >= 2 && !ag_wait(&cdone[ci & 1u], ((ci >> 1) & 1u) ^ 1u)) { ok = false; break; }
           if (!ag_wait(&cfull[ci % S::CHUNKS], (ci / S::CHUNKS) & 1u)) { ok = false; break; }
@@ -345,7 +412,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
           if constexpr (KIND == 16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (i < subs) pr_mma16(d, dp + i * (P_MN ? 128 : 2), dq + i * (Q_MN ? 128 : 2), g.idesc, (kb | i) != 0);
+              if (i < subs) pr_mma16<PAIR>(d, dp + i * (P_MN ? 128 : 2), dq + i * (Q_MN ? 128 : 2), g.idesc, (kb | i) != 0);
           } else {
             const uint32_t tp = tmem + 2 * BN + (ci & 1u) * S::SFC, tq = tp + 16;
             if (kb % S::CHUNK_STAGES == 0) {
@@ -365,20 +432,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             }
             if (kb % S::CHUNK_STAGES == S::CHUNK_STAGES - 1 || kb == nk - 1) ag_commit(&cdone[ci & 1u]);
           }
-          ag_commit(&empty[s]);
+          pr_commit<PAIR>(&empty[s]);
         }
         if (KIND != 16 && (kb % S::CHUNK_STAGES == S::CHUNK_STAGES - 1 || kb == nk - 1)) ++ci;
       }
-      if (one) ag_commit(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
+      if (one) pr_commit<PAIR>(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
     }
     if (one) ag_commit(done);   // every issued MMA has completed before the tensor memory is freed
     if (!ag_wait(done, 0) || !ok) *failed = 1;
-  } else if (warp < 4) {
-    if (HELP) {
+  } else if (warp == 2 || warp == 3) {
+    if (KIND != 16 || (RELAY && warp - 2 < RELAYS)) {
       const int h = tid - 64;
       uint32_t it = 0;
-      for (int t = blockIdx.x; t < T.total && ok; t += gridDim.x) {
-        const ProdTile c = prod_tile<FORM, BN>(T, t);
+      for (int t = first; t < T.total && ok; t += step) {
+        const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
         if constexpr (KIND != 16) {
           // rows of w_g and rows of x, whichever is P
           const int w0 = c.f * (FORM == FORM_YT ? PR_BM : BN);
@@ -408,35 +475,39 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ag_smem(&cfull[s])) : "memory");
           }
         } else {
-          const int len = c.r1 - c.r0;
+          const int len = FORM == FORM_DW ? c.r1 - c.r0 : red;
           // every block is passed on, whole or not: a wait that skipped blocks could not tell a
           // stage's next filling from the one after
           for (int k0 = 0; k0 < len; k0 += BK, ++it) {
             const int s = (int)(it % STAGES), tail = len - k0;
             if (!__all_sync(0xffffffffu, pr_wait_long(&full[s], (it / STAGES) & 1u, failed))) { ok = false; break; }
-            if (tail < BK) {
+            if (FORM == FORM_DW && tail < BK) {
               // steps tail .. 63 of every block of 64 values: 128 bytes each, the swizzle stays within them
-              for (int i = h; i < (PR_BM + BN) / 64 * (BK - tail) * 8; i += PR_HELPERS) {
-                const int v = i & 7, step = tail + (i >> 3) % (BK - tail), b = (i >> 3) / (BK - tail);
+              for (int i = h; i < (PR_BM + S::QR) / 64 * (BK - tail) * 8; i += PR_HELPERS) {
+                const int v = i & 7, step_ = tail + (i >> 3) % (BK - tail), b = (i >> 3) / (BK - tail);
                 unsigned char* z = b < PR_BM / 64 ? sP + s * S::P_BYTES + b * 8192 : sQ + s * S::Q_BYTES + (b - PR_BM / 64) * 8192;
-                *(uint4*)(z + step * 128 + v * 16) = make_uint4(0, 0, 0, 0);
+                *(uint4*)(z + step_ * 128 + v * 16) = make_uint4(0, 0, 0, 0);
               }
+              if (PAIR) pr_release_cluster();
               pr_proxy_fence();
             }
             __syncwarp();
-            if (lane == 0) pr_arrive(&fixed[s]);
+            if (lane == 0) {
+              if (PAIR) pr_arrive_leader(&fixed[s]);
+              else pr_arrive(&fixed[s]);
+            }
           }
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       if (!ok) *failed = 1;
     }
-  } else {   // results
+  } else if (warp >= 4) {   // results
     const int ew = warp - 4, quarter = ew & 3, half = ew >> 2;
     unsigned char* stg = staging + ew * 2048;
     uint32_t j = 0;
-    for (int t = blockIdx.x; t < T.total; t += gridDim.x, ++j) {
-      const ProdTile c = prod_tile<FORM, BN>(T, t);
+    for (int t = first; t < T.total; t += step, ++j) {
+      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
       const uint32_t acc = j & 1u;
       if (!__all_sync(0xffffffffu, pr_wait_long(&tfull[acc], (j >> 1) & 1u, failed) && !*failed)) {
         if (lane == 0) *failed = 1;
@@ -446,7 +517,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       const bool none = FORM == FORM_DW && c.r1 == c.r0;   // an empty group: zeros
       const uint32_t d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
       // tile's place in y: rows row0 .. row_lim - 1, columns col0 .. col_lim - 1
-      const int row0 = FORM == FORM_DW ? c.f % g.p_tiles * PR_BM : c.r0, row_lim = FORM == FORM_DW ? g.n : c.r1;
+      const int row0 = (FORM == FORM_DW ? c.f % g.p_tiles * RT : c.r0) + rank * PR_BM, row_lim = FORM == FORM_DW ? g.n : c.r1;
       const int col0 = FORM == FORM_DW ? c.f / g.p_tiles * BN : c.f * (FORM == FORM_YT ? PR_BM : BN);
       const int col_lim = FORM == FORM_Y || FORM == FORM_YT ? g.n : g.k;
       const int64_t y0 = FORM == FORM_DW ? (int64_t)c.g * g.y_stride : 0;
@@ -531,15 +602,22 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       }
       ag_fence_before();
       __syncwarp();
-      if (lane == 0) pr_arrive(&tempty[acc]);
+      if (lane == 0) {
+        if (PAIR) pr_arrive_leader(&tempty[acc]);
+        else pr_arrive(&tempty[acc]);
+      }
     }
   }
   __syncwarp();
   ag_fence_before();
   __syncthreads();
+  pr_cluster_sync<PAIR>();   // neither CTA leaves while the other's MMAs or arrivals may still reach it
   if (tid == 0 && *failed && g.err) atomicOr(g.err, SMG_PROD_TIMEOUT);
   if (warp == 2) {
     ag_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
   }
 }

@@ -66,14 +66,15 @@ struct Operands {
   int64_t a_len, b_len;   // values of a row (microscaled: bytes)
 };
 
-template <int KIND, int BN, int FORM>
+template <int KIND, int BN, int FORM, bool PAIR = false>
 static int launch(const char* who, const Operands& o, ProdArgs g, int type, cudaStream_t st) {
-  using S = ProdShape<KIND, BN>;
+  using S = ProdShape<KIND, BN, PAIR>;
   constexpr bool bytes = KIND != 16;
   const int wide = FORM == FORM_Y || FORM == FORM_YT ? g.n : g.k;
-  g.p_tiles = FORM == FORM_YT ? (g.n + PR_BM - 1) / PR_BM : FORM == FORM_DW ? (g.n + PR_BM - 1) / PR_BM : 1;
+  const int pr = PAIR ? 2 * PR_BM : PR_BM;   // rows of P in a tile
+  g.p_tiles = FORM == FORM_YT || FORM == FORM_DW ? (g.n + pr - 1) / pr : 1;
   g.q_tiles = FORM == FORM_YT ? 1 : (wide + BN - 1) / BN;
-  const int64_t per = (int64_t)g.p_tiles * g.q_tiles, rt = FORM == FORM_YT ? BN : PR_BM;
+  const int64_t per = (int64_t)g.p_tiles * g.q_tiles, rt = FORM == FORM_YT ? BN : pr;
   const int64_t row_tiles = FORM == FORM_DW ? g.n_groups : g.rows / rt + std::min(g.n_groups, g.rows);   // at most
   if (row_tiles * per > 0x7fffffff) return fail(SMG_ERR_CAPACITY, "%s: too many tiles for one call", who);
   CUtensorMap tA, tB;
@@ -84,26 +85,38 @@ static int launch(const char* who, const Operands& o, ProdArgs g, int type, cuda
   } else {
     r = encode(who, &tA, o.a, bytes, o.a_len, g.rows, 0, o.lda, 0, FORM == FORM_YT ? BN : PR_BM);
     if (!r) r = encode(who, &tB, o.b, bytes, o.b_len, g.n, g.n_groups, o.ldb, g.n_groups > 1 ? o.b_stride : o.ldb * (int64_t)g.n,
-                       FORM == FORM_Y ? BN : FORM == FORM_YT ? PR_BM : 64);
+                       FORM == FORM_Y ? S::QR : FORM == FORM_YT ? PR_BM : 64);
   }
   if (r) return r;
   // instruction descriptor: operand types (f16 0, bf16 1 with 32-bit sums in bits 4-5; e4m3 0, e2m1 1 with
   // power-of-two scales in bit 23) at 7 and 10, MN-major P and Q at 15 and 16, BN / 8 at 17, 128 / 16 at 24
   const uint32_t fmt = KIND == 16 ? (type == SMG_EMB_BF16) : KIND == 4;
-  g.idesc = fmt << 7 | fmt << 10 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(PR_BM >> 4) << 24 | (KIND == 16 ? 1u << 4 : 1u << 23) |
+  g.idesc = fmt << 7 | fmt << 10 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(pr >> 4) << 24 | (KIND == 16 ? 1u << 4 : 1u << 23) |
             (FORM == FORM_DW ? 1u << 15 : 0u) | (FORM == FORM_DX || FORM == FORM_DW ? 1u << 16 : 0u);
   g.y_vec = rows16(g.y, g.ldy, g.y_type) && (FORM != FORM_DW || g.y_stride * size_of(g.y_type) % 16 == 0);
-  static std::atomic<uint64_t> ready;   // devices on which this kernel has its shared memory
+  static std::atomic<uint64_t> ready{0};   // devices on which this kernel has its shared memory
   int dev = 0;
   const int sms = sm_count(&dev);
   if (!sms) return fail(SMG_ERR_DEVICE, "%s: no usable device (%s)", who, cudaGetErrorString(cudaGetLastError()));
   if (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    const cudaError_t e = cudaFuncSetAttribute(k_prod<KIND, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(k_prod<KIND, BN, FORM, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return fail(SMG_ERR_DEVICE, "%s: %s", who, cudaGetErrorString(e));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  k_prod<KIND, BN, FORM><<<(unsigned)std::min<int64_t>(sms, row_tiles * per), PR_THREADS, S::SMEM, st>>>(tA, tB, g);
-  return launched(who);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(PAIR ? 2 * std::min<int64_t>(sms / 2, row_tiles * per) : std::min<int64_t>(sms, row_tiles * per)));
+  cfg.blockDim = dim3(PR_THREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = PAIR ? 2 : 1;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_prod<KIND, BN, FORM, PAIR>, tA, tB, g);
+  if (e != cudaSuccess) return fail(SMG_ERR_DEVICE, "%s: %s", who, cudaGetErrorString(e));
+  return SMG_OK;
 }
 
 static ProdArgs prod_fill(const int32_t* off, int n_groups, int rows, int n, int k, void* y, int64_t ldy, int64_t y_stride, int y_type,
@@ -116,6 +129,7 @@ static ProdArgs prod_fill(const int32_t* off, int n_groups, int rows, int n, int
 
 // Few rows a group: their tile is the narrow side (FORM_YT), so that the MMAs are not mostly over rows
 // that are not there.
+static bool many_rows(int rows, int n_groups) { return (int64_t)rows >= 512ll * n_groups; }
 static bool few_rows(int rows, int n_groups) { return (int64_t)rows <= 32ll * n_groups; }
 
 extern "C" {
@@ -133,6 +147,7 @@ int smg_group_product(const void* x, int64_t ldx, const void* w, int64_t ldw, in
   const ProdArgs g = prod_fill(off, n_groups, rows, n, k, y, ldy, 0, y_type, err);
   const Operands o = {x, w, ldx, ldw, w_stride, k, k};
   if (few_rows(rows, n_groups)) return launch<16, 32, FORM_YT>(who, o, g, type, (cudaStream_t)stream);
+  if (many_rows(rows, n_groups)) return launch<16, 256, FORM_Y, true>(who, o, g, type, (cudaStream_t)stream);
   return launch<16, 256, FORM_Y>(who, o, g, type, (cudaStream_t)stream);
 }
 
@@ -149,6 +164,7 @@ int smg_group_product_dx(const void* dy, int64_t lddy, const void* w, int64_t ld
   if (rows == 0) return SMG_OK;
   const ProdArgs g = prod_fill(off, n_groups, rows, n, k, dx, lddx, 0, dx_type, err);
   const Operands o = {dy, w, lddy, ldw, w_stride, n, k};
+  if (many_rows(rows, n_groups)) return launch<16, 256, FORM_DX, true>(who, o, g, type, (cudaStream_t)stream);
   return launch<16, 256, FORM_DX>(who, o, g, type, (cudaStream_t)stream);
 }
 
@@ -169,6 +185,7 @@ int smg_group_product_dw(const void* dy, int64_t lddy, const void* x, int64_t ld
     o.lda = (n + 7) / 8 * 8;
     o.ldb = (k + 7) / 8 * 8;
   }
+  if (many_rows(rows, n_groups)) return launch<16, 256, FORM_DW, true>(who, o, g, type, (cudaStream_t)stream);
   return launch<16, 256, FORM_DW>(who, o, g, type, (cudaStream_t)stream);
 }
 

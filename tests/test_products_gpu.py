@@ -70,6 +70,26 @@ def test_grouped_sizes_of_every_variant(rows, groups):
     check_products(c, 384, 192, BF)
 
 
+@pytest.mark.parametrize("counts", [[700, 0, 1500, 513], [1, 3000], [2049], [0, 256, 1800, 255, 257]])
+@pytest.mark.parametrize("n,k", [(520, 264), (256, 1000), (72, 2048)])
+def test_grouped_many_rows(counts, n, k):
+    """Groups of more rows than a tile of two CTAs has, sizes that no tile divides."""
+    check_products(counts, n, k, HF if n == 256 else BF, FP if n == 72 else None)
+
+
+def test_many_rows_do_not_leak():
+    """NaN in one large group's rows stays there: tiles of two CTAs that reach into the next group."""
+    c = [900, 700, 0, 800]
+    off = R.offsets(c, "cuda")
+    x, w, dy = rnd(2400, 264), rnd(4, 392, 264), rnd(2400, 392)
+    want = P.grouped(x, w, off), P.grouped_dx(dy, w, off), P.grouped_dw(dy, x, off)
+    x[900:1600], dy[900:1600], w[1], w[2] = (float("nan"),) * 4
+    y, dx, dw = P.grouped(x, w, off), P.grouped_dx(dy, w, off), P.grouped_dw(dy, x, off)
+    for got, ref in ((y, want[0]), (dx, want[1])):
+        assert torch.equal(got[:900], ref[:900]) and torch.equal(got[1600:], ref[1600:]) and got[900:1600].isnan().all()
+    assert torch.equal(dw[0], want[2][0]) and torch.equal(dw[3], want[2][3]) and not dw[2].any() and dw[1].isnan().all()
+
+
 def test_one_group_without_offsets():
     x, w = rnd(50, 96), rnd(1, 40, 96)
     R.near(P.grouped(x, w, None, FP), R.y64(x, w, None), R.y64(x.abs(), w.abs(), None), 96, "y")

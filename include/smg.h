@@ -560,8 +560,8 @@ int smg_assoc_stamps(smg_assoc* a, int enable, int64_t* out16);
  * off[g] .. off[g+1] - 1 (off: n_groups + 1 device entries, off[0] = 0, off[n_groups] = rows, never
  * decreasing; a group may be empty).  off = NULL means one group of all rows (n_groups = 1).
  * err (may be NULL) is a device word that gets SMG_PROD_TIMEOUT or'ed in when a wait inside the
- * kernel ran out and SMG_PROD_OFFSETS when off breaks these rules (every group is then taken as
- * empty: nothing is computed, and dw is zeros).  n_groups <= 1024. */
+ * kernel ran out and SMG_PROD_OFFSETS when off breaks these rules (the results are
+ * then unspecified; nothing outside the arrays is read or written).  n_groups <= 1024. */
 #define SMG_PROD_MAX_GROUPS 1024
 enum { SMG_PROD_TIMEOUT = 1, SMG_PROD_OFFSETS = 2 };
 /* y[r][j] = sum_i x[r][i] w[g][j][i] for the rows r of group g: x rows x k, w n_groups x n x k (row j

@@ -205,7 +205,13 @@ DEV bool pr_wait_long(uint64_t* b, uint32_t parity, volatile int* failed) {
 struct ProdTiles {
   const int *beg, *end, *cum;   // first row, row past the last, and first row tile of each group
   int n_groups, fixed;          // tiles of a row tile along the fixed axes
-  int total;
+  int total, first, step;       // this CTA's (pair's) place among the `step` that walk the tiles
+  // The r-th tile of this CTA (>= total: none).  DW's tiles are as long as their groups, the longest first
+  // and every other round of them backwards, so that no CTA has the longest of every round.
+  template <int FORM>
+  DEV int at(int r) const {
+    return r * step + (FORM == FORM_DW && (r & 1) ? step - 1 - first : first);
+  }
 };
 
 struct ProdTile {
@@ -216,16 +222,22 @@ struct ProdTile {
 template <int FORM, int BN, bool PAIR>
 DEV ProdTile prod_tile(const ProdTiles& T, int t) {
   const int u = t / T.fixed;
+  ProdTile r;
+  r.f = t - u * T.fixed;
+  if (FORM == FORM_DW) {        // T.cum: the groups in order of length
+    r.g = T.cum[u];
+    r.r0 = T.beg[r.g];
+    r.r1 = T.end[r.g];
+    return r;
+  }
   int lo = 0, hi = T.n_groups;  // the last group whose first row tile is <= u (empty groups have none)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (T.cum[mid] <= u) lo = mid;
     else hi = mid;
   }
-  ProdTile r;
   r.g = lo;
-  r.f = t - u * T.fixed;
-  r.r0 = T.beg[lo] + (FORM == FORM_DW ? 0 : (u - T.cum[lo]) * (FORM == FORM_YT ? BN : PAIR ? 2 * PR_BM : PR_BM));
+  r.r0 = T.beg[lo] + (u - T.cum[lo]) * (FORM == FORM_YT ? BN : PAIR ? 2 * PR_BM : PR_BM);
   r.r1 = T.end[lo];
   return r;
 }
@@ -319,13 +331,25 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   constexpr uint32_t tmem = 0;
   if (tid == 0 && *tmem_slot != tmem) *failed = 1;
   constexpr int RT = FORM == FORM_YT ? BN : PAIR ? 2 * PR_BM : PR_BM;
-  // which of a pair's 128 rows of P (and of its halves of Q) are this CTA's; the pairs walk the tiles
-  const int rank = PAIR ? (int)pr_rank() : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
-  if (warp == 0) {   // first row tile of every group
+  const int rank = PAIR ? (int)pr_rank() : 0;   // which of a pair's 128 rows of P (and halves of Q) are this CTA's
+  if (FORM == FORM_DW) {   // groups by length (beyond 256 of them, where no single one holds the end up, as they come)
+    for (int i = tid; i < g.n_groups; i += PR_THREADS) {
+      int rank = i;
+      if (g.n_groups <= 256) {
+        const int len = s_end[i] - s_beg[i];
+        rank = 0;
+        for (int o = 0; o < g.n_groups; ++o) {
+          const int other = s_end[o] - s_beg[o];
+          rank += other > len || (other == len && o < i);
+        }
+      }
+      s_cum[rank] = i;
+    }
+  } else if (warp == 0) {   // first row tile of every group
     int at = 0;
     for (int i0 = 0; i0 < g.n_groups; i0 += 32) {
       const int i = i0 + lane;
-      const int own = i >= g.n_groups ? 0 : FORM == FORM_DW ? 1 : (s_end[i] - s_beg[i] + RT - 1) / RT;
+      const int own = i >= g.n_groups ? 0 : (s_end[i] - s_beg[i] + RT - 1) / RT;
       int sum = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -342,7 +366,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   T.beg = s_beg; T.end = s_end; T.cum = s_cum;
   T.n_groups = g.n_groups;
   T.fixed = FORM == FORM_DW ? g.p_tiles * g.q_tiles : FORM == FORM_YT ? g.p_tiles : g.q_tiles;
-  T.total = *failed ? 0 : s_cum[g.n_groups] * T.fixed;
+  T.total = *failed ? 0 : (FORM == FORM_DW ? g.n_groups : s_cum[g.n_groups]) * T.fixed;
+  T.first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+  T.step = PAIR ? gridDim.x >> 1 : gridDim.x;
   const int red = FORM == FORM_DX ? g.n : g.k;   // (DW: the group's rows)
   bool ok = true;
 
@@ -352,7 +378,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   if (warp == 0) {   // loads
     const bool one = pr_elect();
     uint32_t it = 0;
-    for (int t = first; t < T.total && ok; t += step) {
+    for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
       const int nk = ((FORM == FORM_DW ? c.r1 - c.r0 : red) + BK - 1) / BK;
       for (int kb = 0; kb < nk; ++kb, ++it) {
@@ -387,7 +413,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   } else if (warp == 1 && rank == 0) {   // MMAs
     const bool one = pr_elect();
     uint32_t it = 0, j = 0, ci = 0;
-    for (int t = first; t < T.total && ok; t += step, ++j) {
+    for (int t; (t = T.template at<FORM>(j)) < T.total && ok; ++j) {
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
       const int len = FORM == FORM_DW ? c.r1 - c.r0 : red, nk = (len + BK - 1) / BK;
       const uint32_t acc = j & 1u;
@@ -444,7 +470,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     if (KIND != 16 || (RELAY && warp - 2 < RELAYS)) {
       const int h = tid - 64;
       uint32_t it = 0;
-      for (int t = first; t < T.total && ok; t += step) {
+      for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
         const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
         if constexpr (KIND != 16) {
           // rows of w_g and rows of x, whichever is P
@@ -482,11 +508,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             const int s = (int)(it % STAGES), tail = len - k0;
             if (!__all_sync(0xffffffffu, pr_wait_long(&full[s], (it / STAGES) & 1u, failed))) { ok = false; break; }
             if (FORM == FORM_DW && tail < BK) {
-              // steps tail .. 63 of every block of 64 values: 128 bytes each, the swizzle stays within them
-              for (int i = h; i < (PR_BM + S::QR) / 64 * (BK - tail) * 8; i += PR_HELPERS) {
-                const int v = i & 7, step_ = tail + (i >> 3) % (BK - tail), b = (i >> 3) / (BK - tail);
-                unsigned char* z = b < PR_BM / 64 ? sP + s * S::P_BYTES + b * 8192 : sQ + s * S::Q_BYTES + (b - PR_BM / 64) * 8192;
-                *(uint4*)(z + step_ * 128 + v * 16) = make_uint4(0, 0, 0, 0);
+              // steps tail .. of every block of 64 values, up to the last that an MMA reads: 128 bytes each, the
+              // swizzle stays within them
+              const int v = (h & 7) * 16, last = (tail + SUB - 1) / SUB * SUB;
+              for (int k = tail + (h >> 3); k < last; k += PR_HELPERS / 8) {
+#pragma unroll
+                for (int b = 0; b < PR_BM / 64; ++b) *(uint4*)(sP + s * S::P_BYTES + b * 8192 + k * 128 + v) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < S::QR / 64; ++b) *(uint4*)(sQ + s * S::Q_BYTES + b * 8192 + k * 128 + v) = make_uint4(0, 0, 0, 0);
               }
               if (PAIR) pr_release_cluster();
               pr_proxy_fence();
@@ -506,7 +535,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     const int ew = warp - 4, quarter = ew & 3, half = ew >> 2;
     unsigned char* stg = staging + ew * 2048;
     uint32_t j = 0;
-    for (int t = first; t < T.total; t += step, ++j) {
+    for (int t; (t = T.template at<FORM>(j)) < T.total; ++j) {
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
       const uint32_t acc = j & 1u;
       if (!__all_sync(0xffffffffu, pr_wait_long(&tfull[acc], (j >> 1) & 1u, failed) && !*failed)) {
@@ -537,16 +566,36 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             ag_tmem_ld32(d + c0, v);
           }
           if (FORM == FORM_YT) {   // lane: a column of y; v[i]: row row0 + c0 + i
-            const int col = col0 + quarter * 32 + lane;
+            const int colb = col0 + quarter * 32;
+            if (g.y_type == SMG_EMB_F32 || !g.y_vec || colb + 32 > col_lim) {   // 32 neighbouring values of a row a step
+              const int col = colb + lane;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int row = row0 + c0 + i;
-              if (row < row_lim && col < col_lim) {
-                const int64_t at = (int64_t)row * g.ldy + col;
+              for (int i = 0; i < 32; ++i) {
+                const int row = row0 + c0 + i;
+                if (row < row_lim && col < col_lim) {
+                  const int64_t at = (int64_t)row * g.ldy + col;
+                  const float f = __uint_as_float(v[i]);
+                  if (g.y_type == SMG_EMB_F32) ((float*)g.y)[at] = f;
+                  else if (g.y_type == SMG_EMB_BF16) ((__nv_bfloat16*)g.y)[at] = __float2bfloat16_rn(f);
+                  else ((__half*)g.y)[at] = __float2half_rn(f);
+                }
+              }
+            } else {   // through shared memory, 32 rows of 64 bytes: 8 rows x 64 bytes a step
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
                 const float f = __uint_as_float(v[i]);
-                if (g.y_type == SMG_EMB_F32) ((float*)g.y)[at] = f;
-                else if (g.y_type == SMG_EMB_BF16) ((__nv_bfloat16*)g.y)[at] = __float2bfloat16_rn(f);
-                else ((__half*)g.y)[at] = __float2half_rn(f);
+                uint16_t u;
+                if (g.y_type == SMG_EMB_BF16) u = __bfloat16_as_ushort(__float2bfloat16_rn(f));
+                else u = __half_as_ushort(__float2half_rn(f));
+                ((uint16_t*)stg)[i * 32 + lane] = u;
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (lane >> 2), row = row0 + c0 + r;
+                if (row < row_lim)
+                  *(uint4*)((uint16_t*)g.y + (int64_t)row * g.ldy + colb + (lane & 3) * 8) = *(const uint4*)(stg + r * 64 + (lane & 3) * 16);
               }
             }
           } else {

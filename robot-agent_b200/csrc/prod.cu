@@ -2,8 +2,10 @@
 // microscaled rows.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "heads_host.h"
+#include "k_few.cuh"
 #include "k_prod.cuh"
 
 #include <cudaTypedefs.h>
@@ -76,7 +78,7 @@ static int launch(const char* who, const Operands& o, ProdArgs g, int type, cuda
   g.q_tiles = FORM == FORM_YT ? 1 : (wide + BN - 1) / BN;
   const int64_t per = (int64_t)g.p_tiles * g.q_tiles, rt = FORM == FORM_YT ? BN : pr;
   const int64_t row_tiles = FORM == FORM_DW ? g.n_groups : g.rows / rt + std::min(g.n_groups, g.rows);   // at most
-  if (row_tiles * per > 0x7fffffff) return fail(SMG_ERR_CAPACITY, "%s: too many tiles for one call", who);
+  if (row_tiles * per > 0x7ff00000) return fail(SMG_ERR_CAPACITY, "%s: too many tiles for one call", who);
   CUtensorMap tA, tB;
   int r;
   if (FORM == FORM_DW) {
@@ -127,10 +129,23 @@ static ProdArgs prod_fill(const int32_t* off, int n_groups, int rows, int n, int
   return g;
 }
 
-// Few rows a group: their tile is the narrow side (FORM_YT), so that the MMAs are not mostly over rows
-// that are not there.
-static bool many_rows(int rows, int n_groups) { return (int64_t)rows >= 512ll * n_groups; }
-static bool few_rows(int rows, int n_groups) { return (int64_t)rows <= 32ll * n_groups; }
+// Which tile: the one with the least estimated time, (rounds of tiles over the SMs) x (rows of operands
+// that a CTA loads for a tile), since every form is held up by its loads (the 128 x 256 tile of one CTA
+// takes its 384 rows at 55 bytes a cycle and SM, the pair's 256 rows at 45; the MMAs would take 100).  The groups'
+// sizes are known on the device only: they are taken to be spread about their mean, half a tile of each
+// group left over.
+struct TileCost {
+  int64_t rows;
+  int groups, sms;
+  double of(int rt, int64_t fixed, int units, int loaded) const {
+    const double full = (double)std::min<int64_t>(groups, rows), m = rows / full;
+    const double row_tiles = groups == 1 ? std::ceil(m / rt) : full * std::max(1.0, m / rt + 0.5);
+    return std::ceil(row_tiles * fixed / units) * loaded;
+  }
+  double narrow(int64_t wide, int bn) const { return of(bn, (wide + PR_BM - 1) / PR_BM, sms, PR_BM + bn); }    // FORM_YT
+  double single(int64_t wide, int bn) const { return of(PR_BM, (wide + bn - 1) / bn, sms, PR_BM + bn); }
+  double pair(int64_t wide) const { return of(2 * PR_BM, (wide + 255) / 256, sms / 2, 256); }
+};
 
 extern "C" {
 
@@ -146,9 +161,28 @@ int smg_group_product(const void* x, int64_t ldx, const void* w, int64_t ldw, in
   if (rows == 0) return SMG_OK;
   const ProdArgs g = prod_fill(off, n_groups, rows, n, k, y, ldy, 0, y_type, err);
   const Operands o = {x, w, ldx, ldw, w_stride, k, k};
-  if (few_rows(rows, n_groups)) return launch<16, 32, FORM_YT>(who, o, g, type, (cudaStream_t)stream);
-  if (many_rows(rows, n_groups)) return launch<16, 256, FORM_Y, true>(who, o, g, type, (cudaStream_t)stream);
-  return launch<16, 256, FORM_Y>(who, o, g, type, (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  // Up to 8 rows a group, and weights that do not make it a matter of bandwidth: on 1 to 8 rows of one group
+  // (n = k = 1152) 2.8 us against 9, on 24 groups of 512 x 1152 (28 MB) 7.1 against 10.1; on 64 groups (75 MB)
+  // 15.2 against 14.4, and on 64 of 1152 x 1152 42 against 32.
+  if ((int64_t)rows <= FEW_ROWS * (int64_t)n_groups && (int64_t)n_groups * n * k <= 24ll << 20) {
+    const FewArgs a = {off, n_groups, rows, n, k, x, w, ldx, ldw, w_stride, y, ldy, y_type, err};
+    const dim3 grid((n + FEW_W - 1) / FEW_W, n_groups);
+    if (type == SMG_EMB_BF16) k_few<SMG_EMB_BF16><<<grid, FEW_WARPS * 32, 0, st>>>(a);
+    else k_few<SMG_EMB_F16><<<grid, FEW_WARPS * 32, 0, st>>>(a);
+    return launched(who);
+  }
+  int dev;
+  const TileCost c = {rows, n_groups, std::max(sm_count(&dev), 2)};
+  const double t[] = {c.narrow(n, 32), c.narrow(n, 64), c.narrow(n, 128), c.single(n, 192), c.single(n, 256), c.pair(n)};
+  switch (std::min_element(t, t + 6) - t) {
+    case 0: return launch<16, 32, FORM_YT>(who, o, g, type, st);
+    case 1: return launch<16, 64, FORM_YT>(who, o, g, type, st);
+    case 2: return launch<16, 128, FORM_YT>(who, o, g, type, st);
+    case 3: return launch<16, 192, FORM_Y>(who, o, g, type, st);
+    case 4: return launch<16, 256, FORM_Y>(who, o, g, type, st);
+    default: return launch<16, 256, FORM_Y, true>(who, o, g, type, st);
+  }
 }
 
 int smg_group_product_dx(const void* dy, int64_t lddy, const void* w, int64_t ldw, int64_t w_stride, const int32_t* off,
@@ -164,8 +198,16 @@ int smg_group_product_dx(const void* dy, int64_t lddy, const void* w, int64_t ld
   if (rows == 0) return SMG_OK;
   const ProdArgs g = prod_fill(off, n_groups, rows, n, k, dx, lddx, 0, dx_type, err);
   const Operands o = {dy, w, lddy, ldw, w_stride, n, k};
-  if (many_rows(rows, n_groups)) return launch<16, 256, FORM_DX, true>(who, o, g, type, (cudaStream_t)stream);
-  return launch<16, 256, FORM_DX>(who, o, g, type, (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  int dev;
+  const TileCost c = {rows, n_groups, std::max(sm_count(&dev), 2)};
+  const double t[] = {c.single(k, 128), c.single(k, 192), c.single(k, 256), c.pair(k)};
+  switch (std::min_element(t, t + 4) - t) {
+    case 0: return launch<16, 128, FORM_DX>(who, o, g, type, st);
+    case 1: return launch<16, 192, FORM_DX>(who, o, g, type, st);
+    case 2: return launch<16, 256, FORM_DX>(who, o, g, type, st);
+    default: return launch<16, 256, FORM_DX, true>(who, o, g, type, st);
+  }
 }
 
 int smg_group_product_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int32_t* off, int n_groups, int rows,
@@ -185,8 +227,19 @@ int smg_group_product_dw(const void* dy, int64_t lddy, const void* x, int64_t ld
     o.lda = (n + 7) / 8 * 8;
     o.ldb = (k + 7) / 8 * 8;
   }
-  if (many_rows(rows, n_groups)) return launch<16, 256, FORM_DW, true>(who, o, g, type, (cudaStream_t)stream);
-  return launch<16, 256, FORM_DW>(who, o, g, type, (cudaStream_t)stream);
+  // every group has the same tiles, only their lengths differ
+  const cudaStream_t st = (cudaStream_t)stream;
+  int dev;
+  const int sms = std::max(sm_count(&dev), 2);
+  const auto cost = [&](int rt, int bn, int units, int loaded) {
+    return std::ceil((double)n_groups * ((n + rt - 1) / rt) * ((k + bn - 1) / bn) / units) * loaded;
+  };
+  const double t[] = {cost(128, 128, sms, 256), cost(128, 256, sms, 384), cost(256, 256, sms / 2, 256)};
+  switch (std::min_element(t, t + 3) - t) {
+    case 0: return launch<16, 128, FORM_DW>(who, o, g, type, st);
+    case 1: return launch<16, 256, FORM_DW>(who, o, g, type, st);
+    default: return launch<16, 256, FORM_DW, true>(who, o, g, type, st);
+  }
 }
 
 int smg_mx_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales,
@@ -205,9 +258,15 @@ int smg_mx_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_
   const int64_t len = (int64_t)m.kb * 4 * bits;
   const Operands o = {a_codes, b_codes, len, len, len * n, len, len};
   const cudaStream_t st = (cudaStream_t)stream;
-  if (few_rows(rows, n_groups))
-    return bits == 4 ? launch<4, 32, FORM_YT>(who, o, g, 0, st) : launch<8, 32, FORM_YT>(who, o, g, 0, st);
-  return bits == 4 ? launch<4, 192, FORM_Y>(who, o, g, 0, st) : launch<8, 192, FORM_Y>(who, o, g, 0, st);
+  int dev;
+  const TileCost c = {rows, n_groups, std::max(sm_count(&dev), 2)};
+  const double t[] = {c.narrow(n, 32), c.narrow(n, 64), c.narrow(n, 128), c.single(n, 192)};
+  switch (std::min_element(t, t + 4) - t) {
+    case 0: return bits == 4 ? launch<4, 32, FORM_YT>(who, o, g, 0, st) : launch<8, 32, FORM_YT>(who, o, g, 0, st);
+    case 1: return bits == 4 ? launch<4, 64, FORM_YT>(who, o, g, 0, st) : launch<8, 64, FORM_YT>(who, o, g, 0, st);
+    case 2: return bits == 4 ? launch<4, 128, FORM_YT>(who, o, g, 0, st) : launch<8, 128, FORM_YT>(who, o, g, 0, st);
+    default: return bits == 4 ? launch<4, 192, FORM_Y>(who, o, g, 0, st) : launch<8, 192, FORM_Y>(who, o, g, 0, st);
+  }
 }
 
 }   // extern "C"

@@ -18,11 +18,6 @@ static inline int fail(int code, const char* fmt, ...) {
   return smg_set_error(code, msg);
 }
 
-static inline int launched(const char* who) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? SMG_OK : fail(SMG_ERR_DEVICE, "%s: %s", who, cudaGetErrorString(e));
-}
-
 static inline bool on16(const void* p) { return !((uintptr_t)p & 15); }
 static inline bool type_ok(int t) { return t == SMG_EMB_F32 || t == SMG_EMB_BF16 || t == SMG_EMB_F16; }
 static inline int size_of(int t) { return t == SMG_EMB_F32 ? 4 : 2; }
@@ -55,4 +50,21 @@ static inline MxDiv mx_div(int per) {
   while ((1ll << shift) < per) ++shift;
   const MxDiv d = {(uint32_t)per, (uint32_t)(((1ull << (31 + shift)) + (uint32_t)per - 1) / (uint32_t)per), shift};
   return d;
+}
+
+// A launch that may be set up while the kernel before it in the stream still runs (heads_wait).
+template <typename... P, typename... A>
+static inline int launch_next(const char* who, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  return e == cudaSuccess ? SMG_OK : fail(SMG_ERR_DEVICE, "%s: %s", who, cudaGetErrorString(e));
 }

@@ -53,6 +53,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) k_few(FewArgs a) {
   typedef typename Elem<TYPE>::T T;
   __shared__ float part[FEW_WARPS][FEW_ROWS][FEW_W + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y, j0 = blockIdx.x * FEW_W;
+  heads_next();
+  heads_wait();
   int r0 = 0, r1 = a.rows;
   if (a.off) {
     r0 = a.off[g];

@@ -19,6 +19,11 @@
 #define DEV __device__ __forceinline__
 #endif
 
+// Programmatic launch: a kernel may be set up while the one before it in the stream still runs.  It
+// touches global memory only after heads_wait(), which returns when that one is complete, its writes included.
+DEV void heads_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+DEV void heads_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- 8 consecutive values of a row <-> 8 floats ----
 template <int TYPE>
 struct Elem;
@@ -244,6 +249,8 @@ DEV void mx_place(int64_t t, int64_t n, const MxDiv& d, int64_t& row, int& j) {
 #define MX_EACH 4
 template <int TYPE, int BITS, bool VEC>
 __global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::T* x, int64_t ldx, int64_t n, MxDiv div, MxOut o) {
+  heads_next();
+  heads_wait();
   const int64_t t0 = (int64_t)blockIdx.x * (256 * MX_EACH) + threadIdx.x;
   Raw8<TYPE> raw[MX_EACH];
   int64_t row[MX_EACH];
@@ -267,6 +274,8 @@ __global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::
 // MX_EACH parts of 8 values a thread
 template <int TYPE, int BITS>
 __global__ void __launch_bounds__(256) k_mx_values(MxOut o, int64_t n, MxDiv div, typename Elem<TYPE>::T* out, int64_t ld, bool vec) {
+  heads_next();
+  heads_wait();
   const int64_t t0 = (int64_t)blockIdx.x * (256 * MX_EACH) + threadIdx.x;
 #pragma unroll
   for (int i = 0; i < MX_EACH; ++i) {

@@ -58,6 +58,8 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_add(NormArgs a) {
   const int sub = threadIdx.x / (32 * WARPS), t = threadIdx.x % (32 * WARPS);
   const int64_t row = (int64_t)blockIdx.x * NORM_ROWS(WARPS) + sub;
   if (row >= a.rows) return;   // all warps of a row together
+  heads_next();
+  heads_wait();
   float h[NV][8];
   {
     Raw8<TYPE> x[NV], r[NV];
@@ -112,6 +114,8 @@ __global__ void __launch_bounds__(NORM_THREADS, NV <= 3 ? 2 : 1) k_norm_add_bwd(
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int k = 0; k < 8; ++k) dg[i][k] = 0.f;
+  heads_next();
+  heads_wait();
   const int64_t step = (int64_t)gridDim.x * NORM_ROWS(WARPS);
   for (int64_t row = (int64_t)blockIdx.x * NORM_ROWS(WARPS) + sub; row < a.rows; row += step) {
     Raw8<TYPE> x[NV], r[NV], y[NV], d[NV];
@@ -175,6 +179,8 @@ __global__ void __launch_bounds__(NORM_THREADS, NV <= 3 ? 2 : 1) k_norm_add_bwd(
 __global__ void __launch_bounds__(1024) k_norm_dgain(const float* part, int n_part, int dim, float* dgain) {
   __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  heads_next();
+  heads_wait();
   float v = 0.f;
   if (c < dim)
     for (int p = w; p < n_part; p += 32) v += part[(int64_t)p * dim + c];

@@ -308,6 +308,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
   }
+  heads_next();
+  heads_wait();   // barriers and tensor memory are set up; from here on global memory is read
   // groups: offsets that break the rules are reported, and every group is then taken as empty
   int bad = 0;
   for (int i = tid; i < g.n_groups; i += PR_THREADS) {

@@ -110,12 +110,14 @@ static int launch(const char* who, const Operands& o, ProdArgs g, int type, cuda
   cfg.blockDim = dim3(PR_THREADS);
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = PAIR ? 2 : 1;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // as launch_next
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = PAIR ? 1 : 0;
+  cfg.numAttrs = PAIR ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, k_prod<KIND, BN, FORM, PAIR>, tA, tB, g);
   if (e != cudaSuccess) return fail(SMG_ERR_DEVICE, "%s: %s", who, cudaGetErrorString(e));
   return SMG_OK;
@@ -168,9 +170,7 @@ int smg_group_product(const void* x, int64_t ldx, const void* w, int64_t ldw, in
   if ((int64_t)rows <= FEW_ROWS * (int64_t)n_groups && (int64_t)n_groups * n * k <= 24ll << 20) {
     const FewArgs a = {off, n_groups, rows, n, k, x, w, ldx, ldw, w_stride, y, ldy, y_type, err};
     const dim3 grid((n + FEW_W - 1) / FEW_W, n_groups);
-    if (type == SMG_EMB_BF16) k_few<SMG_EMB_BF16><<<grid, FEW_WARPS * 32, 0, st>>>(a);
-    else k_few<SMG_EMB_F16><<<grid, FEW_WARPS * 32, 0, st>>>(a);
-    return launched(who);
+    return launch_next(who, type == SMG_EMB_BF16 ? k_few<SMG_EMB_BF16> : k_few<SMG_EMB_F16>, grid, FEW_WARPS * 32, 0, st, a);
   }
   int dev;
   const TileCost c = {rows, n_groups, std::max(sm_count(&dev), 2)};

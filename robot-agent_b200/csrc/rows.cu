@@ -33,15 +33,13 @@ int smg_mx_quantise(const void* x, int64_t ldx, int rows, int k, int type, int b
   const bool vec = rows16(x, ldx, type) && k % 8 == 0;
   unsigned grid;
   if (int r = mx_blocks(who, n, &grid)) return r;
-#define CALL(TY)                                                                                                              \
-  const Elem<TY>::T* p = (const Elem<TY>::T*)x;                                                                               \
-  if (vec && bits == 4) k_mx_quantise<TY, 4, true><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, mx_div(o.pitch * 4), o);                      \
-  else if (vec) k_mx_quantise<TY, 8, true><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, mx_div(o.pitch * 4), o);                              \
-  else if (bits == 4) k_mx_quantise<TY, 4, false><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, mx_div(o.pitch * 4), o);                       \
-  else k_mx_quantise<TY, 8, false><<<grid, 256, 0, (cudaStream_t)stream>>>(p, ldx, n, mx_div(o.pitch * 4), o)
+  const cudaStream_t st = (cudaStream_t)stream;
+#define CALL(TY)                                                                                              \
+  const auto f = bits == 4 ? (vec ? k_mx_quantise<TY, 4, true> : k_mx_quantise<TY, 4, false>)                 \
+                           : (vec ? k_mx_quantise<TY, 8, true> : k_mx_quantise<TY, 8, false>);                \
+  return launch_next(who, f, grid, 256, 0, st, (const Elem<TY>::T*)x, ldx, n, mx_div(o.pitch * 4), o)
   BY_TYPE(type, CALL);
 #undef CALL
-  return launched(who);
 }
 
 int smg_mx_values(const uint8_t* codes, const uint8_t* scales, int rows, int k, int bits, void* out, int64_t ld, int out_type,
@@ -57,12 +55,11 @@ int smg_mx_values(const uint8_t* codes, const uint8_t* scales, int rows, int k, 
   const bool vec = rows16(out, ld, out_type);
   unsigned grid;
   if (int r = mx_blocks(who, n, &grid)) return r;
-#define CALL(TY)                                                                                                  \
-  if (bits == 4) k_mx_values<TY, 4><<<grid, 256, 0, (cudaStream_t)stream>>>(o, n, mx_div(o.kb * 4), (Elem<TY>::T*)out, ld, vec);      \
-  else k_mx_values<TY, 8><<<grid, 256, 0, (cudaStream_t)stream>>>(o, n, mx_div(o.kb * 4), (Elem<TY>::T*)out, ld, vec)
+#define CALL(TY)                                                                                              \
+  return launch_next(who, bits == 4 ? k_mx_values<TY, 4> : k_mx_values<TY, 8>, grid, 256, 0, (cudaStream_t)stream, o, n, \
+                     mx_div(o.kb * 4), (Elem<TY>::T*)out, ld, vec)
   BY_TYPE(out_type, CALL);
 #undef CALL
-  return launched(who);
 }
 
 // ------------------------------------------------------------------ residual norm
@@ -121,13 +118,10 @@ int smg_norm_add(const void* x, int64_t ldx, const void* r, int64_t ldr, const f
   const bool vec = dim % 8 == 0 && rows16(x, ldx, type) && (!r || rows16(r, ldr, type)) && (!h || rows16(h, ldh, type)) && on16(gain);
   a.mx = mx_rows(dim, codes, scales, values);
   const int steps = (a.mx.pitch * 4 + 31) / 32;   // of 256 values, the scales' padding included
-  const cudaStream_t st = (cudaStream_t)stream;
-#define LAUNCH(T, W, NV)                                                                         \
-  const unsigned grid = (unsigned)((rows + NORM_ROWS(W) - 1) / NORM_ROWS(W));                    \
-  if (bits == 4 && vec) k_norm_add<T, 4, W, NV, true><<<grid, NORM_THREADS, 0, st>>>(a);         \
-  else if (bits == 4) k_norm_add<T, 4, W, NV, false><<<grid, NORM_THREADS, 0, st>>>(a);          \
-  else if (vec) k_norm_add<T, 8, W, NV, true><<<grid, NORM_THREADS, 0, st>>>(a);                 \
-  else k_norm_add<T, 8, W, NV, false><<<grid, NORM_THREADS, 0, st>>>(a)
+#define LAUNCH(T, W, NV)                                                                                      \
+  const auto f = bits == 4 ? (vec ? k_norm_add<T, 4, W, NV, true> : k_norm_add<T, 4, W, NV, false>)           \
+                           : (vec ? k_norm_add<T, 8, W, NV, true> : k_norm_add<T, 8, W, NV, false>);          \
+  return launch_next(who, f, (unsigned)((rows + NORM_ROWS(W) - 1) / NORM_ROWS(W)), NORM_THREADS, 0, (cudaStream_t)stream, a)
 #define CALL32(W, NV) LAUNCH(SMG_EMB_F32, W, NV)
 #define CALLBF(W, NV) LAUNCH(SMG_EMB_BF16, W, NV)
 #define CALLHF(W, NV) LAUNCH(SMG_EMB_F16, W, NV)
@@ -135,7 +129,6 @@ int smg_norm_add(const void* x, int64_t ldx, const void* r, int64_t ldr, const f
   else if (type == SMG_EMB_BF16) BY_STEPS5(steps, CALLBF);
   else BY_STEPS5(steps, CALLHF);
 #undef LAUNCH
-  return launched(who);
 }
 
 int64_t smg_norm_add_bwd_work(int dim) { return dim < 1 ? 0 : (int64_t)NORM_PARTS * dim * 4; }
@@ -158,21 +151,20 @@ int smg_norm_add_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
                    (!dh || rows16(dh, lddh, type)) && rows16(dx, lddx, type) && on16(gain);
   const cudaStream_t st = (cudaStream_t)stream;
   const int steps = (dim + 255) / 256;
-  int parts = 0;
+  int parts = 0, e = SMG_OK;
   if (rows > 0) {
 #define LAUNCH(T, W, NV)                                                                         \
   parts = (rows + NORM_ROWS(W) - 1) / NORM_ROWS(W);                                              \
   if (parts > NORM_PARTS) parts = NORM_PARTS;                                                    \
   const int sm = W < 8 ? NORM_ROWS(W) * dim * 4 : 0;                                             \
-  if (vec) k_norm_add_bwd<T, W, NV, true><<<parts, NORM_THREADS, sm, st>>>(a);                   \
-  else k_norm_add_bwd<T, W, NV, false><<<parts, NORM_THREADS, sm, st>>>(a)
+  e = launch_next(who, vec ? k_norm_add_bwd<T, W, NV, true> : k_norm_add_bwd<T, W, NV, false>, parts, NORM_THREADS, sm, st, a)
     if (type == SMG_EMB_F32) BY_STEPS2(steps, CALL32);
     else if (type == SMG_EMB_BF16) BY_STEPS3(steps, CALLBF);
     else BY_STEPS3(steps, CALLHF);
 #undef LAUNCH
   }
-  k_norm_dgain<<<(dim + 31) / 32, 1024, 0, st>>>(a.part, parts, dim, dgain);
-  return launched(who);
+  if (e) return e;
+  return launch_next(who, k_norm_dgain, (dim + 31) / 32, 1024, 0, st, a.part, parts, dim, dgain);
 }
 
 }   // extern "C"

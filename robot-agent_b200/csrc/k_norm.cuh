@@ -42,6 +42,17 @@ DEV float row_sum(float v, float* scr, int sub) {
   return v;
 }
 
+// 1 / sqrt(ss / dim + eps) as a float and what it lacks (both together good to about 2^-45): the float's
+// residual 1 - (v + ve) r^2, with v + ve the argument before its roundings, halved, corrects it (one Newton step).
+DEV float rstd_of(float ss, float dim, float eps, float& low) {
+  const float q = ss / dim, qe = __fmaf_rn(-q, dim, ss) / dim;
+  const float v = q + eps, b = v - q, ve = ((q - (v - b)) + (eps - b)) + qe;
+  const float r = 1.f / sqrtf(v), t = v * r, te = __fmaf_rn(v, r, -t);
+  const float e = __fmaf_rn(-ve * r, r, __fmaf_rn(-te, r, __fmaf_rn(-t, r, 1.f)));
+  low = 0.5f * r * e;
+  return r;
+}
+
 // gain of 8 columns; VEC: on 16 bytes, n a multiple of 8
 template <bool VEC>
 DEV void gain8(const float* p, int n, float (&g)[8]) {
@@ -80,13 +91,18 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_add(NormArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) h[i][k] = a.r ? x[i].get(k) + r[i].get(k) : x[i].get(k);
   }
-  float ss = 0.f;
+  float sq[8];   // 8 short sums, then their tree: fewer roundings than one long sum
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int k = 0; k < 8; ++k) sq[k] = h[0][k] * h[0][k];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ss = __fmaf_rn(h[i][k], h[i][k], ss);
-  ss = row_sum<WARPS>(ss, scr[sub], sub);
-  const float rstd = 1.f / sqrtf(ss / (float)a.dim + a.eps);
+  for (int i = 1; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sq[k] = __fmaf_rn(h[i][k], h[i][k], sq[k]);
+  const float ss = row_sum<WARPS>(((sq[0] + sq[1]) + (sq[2] + sq[3])) + ((sq[4] + sq[5]) + (sq[6] + sq[7])), scr[sub], sub);
+  // The codes' rounding turns an error of the last place into one of a code, so 1 / rms goes in two parts: what
+  // remains are the two products' own roundings (carrying those on too changed next to no code).
+  float low;
+  const float rstd = rstd_of(ss, (float)a.dim, a.eps, low);
   if (a.rstd && t == 0) a.rstd[row] = rstd;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -95,7 +111,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_add(NormArgs a) {
     float g[8];
     gain8<VEC>(a.gain + c, n, g);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * rstd * g[k];
+    for (int k = 0; k < 8; ++k) h[i][k] = __fmaf_rn(h[i][k], rstd, h[i][k] * low) * g[k];
     mx_emit<BITS>(a.mx, row, j, h[i]);
   }
 }

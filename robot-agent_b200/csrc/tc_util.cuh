@@ -38,8 +38,10 @@ DEV bool ag_try_wait(uint64_t* b, uint32_t parity) {
   return ok != 0;
 }
 
-// bounded wait on phase `parity`; false after AG_WAIT_NS
+// bounded wait on phase `parity`; false after AG_WAIT_NS.  The clock is read only when the first try has
+// failed: reading it takes as long as several MMAs.
 DEV bool ag_wait(uint64_t* b, uint32_t parity) {
+  if (ag_try_wait(b, parity)) return true;
   const uint64_t t0 = ag_now();
   for (uint32_t i = 0;; ++i) {
     if (ag_try_wait(b, parity)) return true;

@@ -303,6 +303,12 @@ def test_scores_of_one_bank(bits, rows, n, k):
     check_scores([rows], n, k, bits)
 
 
+@pytest.mark.parametrize("bits,k", [(4, 1152), (4, 130), (8, 600), (8, 96)])
+def test_scores_many_tiles_of_short_rows(bits, k):
+    """Runs of tiles over the same rows: several row tiles, an empty group and ragged ends in one CTA's run."""
+    check_scores([300, 0, 500, 201], 15001, k, bits, HF)
+
+
 def test_scores_spread_of_magnitudes():
     """Blocks of very different sizes in one row: the scales' exponents add up right."""
     for bits in (4, 8):

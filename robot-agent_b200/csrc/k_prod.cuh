@@ -28,6 +28,8 @@
 //               rows past the group's end in its last block, where the load brought the next group's
 //               rows (in both operands, since zero times NaN is NaN), reported on fixed[s];
 //               Pairs: they pass a landed stage on to the leader's fixed[s];
+//   warp 12     (microscaled rows) copies landed scales to tensor memory, two chunks in turn (cready / cdone): in
+//               the MMA warp the copies and their waits took 300 cycles of the 384 that a stage has;
 //   warps 4-11  read D from tensor memory, round once and store.  Rows past the group's end and
 //               columns past the width are computed and not stored.
 // Pairs (PAIR): two CTAs of a cluster work on one tile of 256 rows of P.  Each loads its own 128 rows
@@ -64,7 +66,7 @@ struct ProdArgs {
 };
 
 #define PR_BM 128
-#define PR_THREADS 384
+#define PR_THREADS(KIND) (KIND == 16 ? 384 : 416)
 #define PR_HELPERS 64
 #define PR_EPI_WARPS 8
 #define PR_SMEM_MAX 232448
@@ -198,6 +200,19 @@ DEV void pr_cluster_sync() {
             : "memory");
 }
 
+// whether the phase is over, without waiting
+DEV bool pr_test(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(ag_smem(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // A wait that may rightly last as long as a whole tile: it goes on while no role has failed (their
 // own waits are bounded).
 DEV bool pr_wait_long(uint64_t* b, uint32_t parity, volatile int* failed) {
@@ -224,6 +239,15 @@ struct ProdTiles {
 struct ProdTile {
   int g, r0, r1;                // group, first row of the tile, row past the group's last
   int f, u;                     // index along the fixed axes; row tile
+  DEV ProdTile uniform() const {
+    ProdTile t;
+    t.g = __shfl_sync(0xffffffffu, g, 0);
+    t.r0 = __shfl_sync(0xffffffffu, r0, 0);
+    t.r1 = __shfl_sync(0xffffffffu, r1, 0);
+    t.f = __shfl_sync(0xffffffffu, f, 0);
+    t.u = __shfl_sync(0xffffffffu, u, 0);
+    return t;
+  }
 };
 
 template <int FORM, int BN, bool PAIR>
@@ -251,7 +275,7 @@ DEV ProdTile prod_tile(const ProdTiles& T, int t) {
 }
 
 template <int KIND, int BN, int FORM, bool PAIR, int HOLD>
-__global__ void __launch_bounds__(PR_THREADS, 1)
+__global__ void __launch_bounds__(PR_THREADS(KIND), 1)
     k_prod(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ ProdArgs g) {
   using S = ProdShape<KIND, BN, PAIR, HOLD>;
   static_assert(!HOLD || (FORM == FORM_Y && !PAIR), "held rows: single CTAs, rows as P");
@@ -277,7 +301,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   uint64_t* cfull = fixed + STAGES;      // microscaled rows: a chunk of scales has landed,
   uint64_t* cempty = cfull + S::CHUNKS;  // has been copied to tensor memory,
   uint64_t* cdone = cempty + S::CHUNKS;  // and the MMAs that use the copy are done
-  uint64_t* tfull = cdone + 2;
+  uint64_t* cready = cdone + 2;          // the copy is in tensor memory
+  uint64_t* tfull = cready + 2;
   uint64_t* tempty = tfull + 2;
   uint64_t* done = tempty + 2;
   uint64_t* pfull = done + 1;            // HOLD: P's rows have landed, and the last MMA on them is done
@@ -297,12 +322,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       ag_mbar_init(&cfull[s], PR_HELPERS);
       ag_mbar_init(&cempty[s], 1);
     }
-    for (int a = 0; a < 2; ++a) ag_mbar_init(&cdone[a], 1);
+    for (int a = 0; a < 2; ++a) {
+      ag_mbar_init(&cdone[a], 1);
+      ag_mbar_init(&cready[a], 1);
+    }
     for (int a = 0; a < 2; ++a) {
       ag_mbar_init(&tfull[a], 1);
       ag_mbar_init(&tempty[a], PR_EPI_WARPS * (PAIR ? 2 : 1));
     }
-    ag_mbar_init(done, 1);
+    ag_mbar_init(done, KIND == 16 ? 1 : 2);
     ag_mbar_init(pfull, 1);
     ag_mbar_init(pfree, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -325,7 +353,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   heads_wait();   // barriers and tensor memory are set up; from here on global memory is read
   // groups: offsets that break the rules are reported, and every group is then taken as empty
   int bad = 0;
-  for (int i = tid; i < g.n_groups; i += PR_THREADS) {
+  for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND)) {
     int a = 0, b = g.rows;
     if (g.off) {
       a = g.off[i];
@@ -340,7 +368,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   ag_fence_after();
   if (bad) {
     if (tid == 0 && blockIdx.x == 0 && g.err) atomicOr(g.err, SMG_PROD_OFFSETS);
-    for (int i = tid; i < g.n_groups; i += PR_THREADS) s_beg[i] = s_end[i] = 0;
+    for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND)) s_beg[i] = s_end[i] = 0;
     __syncthreads();
   }
   constexpr uint32_t tmem = 0;
@@ -348,7 +376,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   constexpr int RT = FORM == FORM_YT ? BN : PAIR ? 2 * PR_BM : PR_BM;
   const int rank = PAIR ? (int)pr_rank() : 0;   // which of a pair's 128 rows of P (and halves of Q) are this CTA's
   if (FORM == FORM_DW) {   // groups by length (beyond 256 of them, where no single one holds the end up, as they come)
-    for (int i = tid; i < g.n_groups; i += PR_THREADS) {
+    for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND)) {
       int rank = i;
       if (g.n_groups <= 256) {
         const int len = s_end[i] - s_beg[i];
@@ -381,7 +409,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   T.beg = s_beg; T.end = s_end; T.cum = s_cum;
   T.n_groups = g.n_groups;
   T.fixed = FORM == FORM_DW ? g.p_tiles * g.q_tiles : FORM == FORM_YT ? g.p_tiles : g.q_tiles;
-  T.total = *failed ? 0 : (FORM == FORM_DW ? g.n_groups : s_cum[g.n_groups]) * T.fixed;
+  T.total = __shfl_sync(0xffffffffu, *failed ? 0 : (FORM == FORM_DW ? g.n_groups : s_cum[g.n_groups]) * T.fixed, 0);
   T.first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
   T.step = PAIR ? gridDim.x >> 1 : gridDim.x;
   T.lo = (int)((int64_t)T.total * T.first / T.step);
@@ -389,18 +417,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   const int red = FORM == FORM_DX ? g.n : g.k;   // (DW: the group's rows)
   bool ok = true;
 
-  // The loads and the MMAs are issued by one elected lane, in code that the whole warp runs: their
-  // operands live in uniform registers, and from a single thread's own code each MMA took 115 cycles to
-  // issue, whatever its width (measured; 32 to 128 run so).
+  // The loads and the MMAs are issued by one elected lane, in code that the whole warp runs and whose branches
+  // the compiler can see to be the warp's (votes, values handed on by a shuffle): their operands live in
+  // uniform registers.  From a single thread's own code each MMA took 115 cycles to issue whatever its
+  // width, a block-scaled one with branches on values out of shared memory 220 (32 to 128 are needed).
+  const auto wait = [](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, ag_wait(b, parity)) != 0; };
   if (warp == 0) {   // loads
     const bool one = pr_elect();
     uint32_t it = 0, np = 0;
     int held = -1;
     for (int r = 0, t; (t = T.template at<FORM, (HOLD > 0)>(r)) < T.total && ok; ++r) {
-      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
+      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t).uniform();
       const int nk = ((FORM == FORM_DW ? c.r1 - c.r0 : red) + BK - 1) / BK;
       if (HOLD && c.u != held) {
-        if (np >= 1 && !ag_wait(pfree, (np - 1) & 1u)) { ok = false; break; }
+        if (np >= 1 && !wait(pfree, (np - 1) & 1u)) { ok = false; break; }
         if (one) {
           ag_expect_tx(pfull, nk * S::P_BYTES);
           for (int kb = 0; kb < nk; ++kb) ag_tma_2d(&tmA, pfull, sP + kb * S::P_BYTES, kb * 128, c.r0);
@@ -410,7 +440,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       }
       for (int kb = 0; kb < nk; ++kb, ++it) {
         const int s = (int)(it % STAGES);
-        if (it >= STAGES && !ag_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
+        if (it >= STAGES && !wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
         unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
         if (!one) continue;
         ag_expect_tx(&full[s], S::STAGE);
@@ -435,20 +465,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       }
     }
     // the last loads must have landed before the CTA ends
-    if (np) ok = ag_wait(pfull, (np - 1) & 1u) && ok;
-    for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j) ok = ag_wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
+    if (np) ok = wait(pfull, (np - 1) & 1u) && ok;
+    for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j) ok = wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
     if (!ok) *failed = 1;
   } else if (warp == 1 && rank == 0) {   // MMAs
     const bool one = pr_elect();
     uint32_t it = 0, j = 0, ci = 0, np = 0;
     int held = -1;
+    bool ready = false;
     for (int t; (t = T.template at<FORM, (HOLD > 0)>(j)) < T.total && ok; ++j) {
-      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
+      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t).uniform();
       const int len = FORM == FORM_DW ? c.r1 - c.r0 : red, nk = (len + BK - 1) / BK;
       const uint32_t acc = j & 1u;
-      if (j >= 2 && !ag_wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
+      if (j >= 2 && !wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
       if (HOLD && c.u != held) {
-        if (!ag_wait(pfull, np & 1u)) { ok = false; break; }
+        if (!wait(pfull, np & 1u)) { ok = false; break; }
         held = c.u;
         ++np;
       }
@@ -458,12 +489,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
         const int s = (int)(it % STAGES);
         const uint32_t ph = (it / STAGES) & 1u;
         const int left = len - kb * BK;
-        if (!ag_wait(RELAY ? &fixed[s] : &full[s], ph)) { ok = false; break; }
-        if (KIND != 16 && kb % S::CHUNK_STAGES == 0) {
-          if (ci >= 2 && !ag_wait(&cdone[ci & 1u], ((ci >> 1) & 1u) ^ 1u)) { ok = false; break; }
-          if (!ag_wait(&cfull[ci % S::CHUNKS], (ci / S::CHUNKS) & 1u)) { ok = false; break; }
-          pr_proxy_fence();   // the scales were written by ordinary copies
-        }
+        uint64_t* landed = RELAY ? fixed : full;
+        if (!__all_sync(0xffffffffu, ready) && !wait(&landed[s], ph)) { ok = false; break; }
+        if (KIND != 16 && kb % S::CHUNK_STAGES == 0 && !wait(&cready[ci & 1u], (ci >> 1) & 1u)) { ok = false; break; }
+        ready = pr_test(&landed[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u);   // the next stage, while this one's MMAs go out
         ag_fence_after();
         const unsigned char *p = sP + (HOLD ? kb : s) * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
         const uint64_t dp = P_MN ? pr_desc_mn(p) : ag_desc(p), dq = Q_MN ? pr_desc_mn(q) : ag_desc(q);
@@ -475,12 +504,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
               if (i < subs) pr_mma16<PAIR>(d, dp + i * (P_MN ? 128 : 2), dq + i * (Q_MN ? 128 : 2), g.idesc, (kb | i) != 0);
           } else {
             const uint32_t tp = tmem + 2 * BN + (ci & 1u) * S::SFC, tq = tp + 16;
-            if (kb % S::CHUNK_STAGES == 0) {
-              const unsigned char* sc = sS + ci % S::CHUNKS * S::CHUNK;
-#pragma unroll
-              for (int i = 0; i < 4 * (1 + S::QCH); ++i) pr_copy_scales(tp + 4 * i, sc + 512 * i);
-              ag_commit(&cempty[ci % S::CHUNKS]);
-            }
             const uint32_t w0 = KIND == 4 ? kb % 2 * 2 : kb % 4;   // the stage's first word of the chunk
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -503,7 +526,29 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       if (one) pr_commit<PAIR>(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
     }
     if (one) ag_commit(done);   // every issued MMA has completed before the tensor memory is freed
-    if (!ag_wait(done, 0) || !ok) *failed = 1;
+    if (!wait(done, 0) || !ok) *failed = 1;
+  } else if (warp == 12) {   // microscaled rows: scales from shared to tensor memory
+    const bool one = pr_elect();
+    uint32_t ci = 0;
+    const int chunks = (red + 511) / 512;
+    for (int r = 0, t; (t = T.template at<FORM, (HOLD > 0)>(r)) < T.total && ok; ++r) {
+      for (int i = 0; i < chunks; ++i, ++ci) {
+        if (ci >= 2 && !wait(&cdone[ci & 1u], ((ci >> 1) & 1u) ^ 1u)) { ok = false; break; }
+        if (!wait(&cfull[ci % S::CHUNKS], (ci / S::CHUNKS) & 1u)) { ok = false; break; }
+        pr_proxy_fence();   // they were written by ordinary copies
+        ag_fence_after();
+        if (one) {
+          const unsigned char* sc = sS + ci % S::CHUNKS * S::CHUNK;
+          const uint32_t tp = tmem + 2 * BN + (ci & 1u) * S::SFC;
+#pragma unroll
+          for (int k = 0; k < 4 * (1 + S::QCH); ++k) pr_copy_scales(tp + 4 * k, sc + 512 * k);
+          ag_commit(&cempty[ci % S::CHUNKS]);
+          ag_commit(&cready[ci & 1u]);
+        }
+      }
+    }
+    if (one) ag_commit(done);
+    if (!ok) *failed = 1;
   } else if (warp == 2 || warp == 3) {
     if (KIND != 16 || (RELAY && warp - 2 < RELAYS)) {
       const int h = tid - 64;
@@ -569,7 +614,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       asm volatile("cp.async.wait_all;" ::: "memory");
       if (!ok) *failed = 1;
     }
-  } else if (warp >= 4) {   // results
+  } else if (warp >= 4 && warp < 12) {   // results
     const int ew = warp - 4, quarter = ew & 3, half = ew >> 2;
     unsigned char* stg = staging + ew * 2048;
     uint32_t j = 0;

@@ -110,7 +110,7 @@ static int launch(const char* who, const Operands& o, ProdArgs g, int type, cuda
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(PAIR ? 2 * std::min<int64_t>(sms / 2, row_tiles * per) : std::min<int64_t>(sms, row_tiles * per)));
-  cfg.blockDim = dim3(PR_THREADS);
+  cfg.blockDim = dim3(PR_THREADS(KIND));
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at[2];

@@ -38,10 +38,6 @@
 // shared memory and reads 48 KB out of it for 512 cycles of MMAs, 192 bytes a cycle where an SM has 128;
 // in a pair it is 32 + 32 KB.
 //
-// Held rows (HOLD): a microscaled product of short rows is held up by what the SMs load, 320 rows for 128 x
-// 192 values of D (8192 x 16384 x 1152 in 4 bits: 1.0 GB, 113 us).  P's 128 rows then stay in shared memory
-// for the CTA's run of neighbouring tiles, and a tile loads Q alone.
-//
 // Every wait is bounded, or goes on only until another role's bounded wait has run out; then the
 // roles run out too, SMG_PROD_TIMEOUT is set, and the CTA waits (bounded) for its own copies and
 // MMAs before it frees the tensor memory.
@@ -73,17 +69,16 @@ struct ProdArgs {
 #define PR_STAGING (PR_EPI_WARPS * 2048)
 #define PR_GROUP_BYTES ((3 * SMG_PROD_MAX_GROUPS + 1) * 4)
 
-// KIND 16: f16 or bf16; 8, 4: microscaled.  HOLD > 0: P's whole rows, up to HOLD stages of them, stay for
-// all tiles of the same rows, and only Q goes through the ring.
-template <int KIND, int BN, bool PAIR, int HOLD>
+// KIND 16: f16 or bf16; 8, 4: microscaled
+template <int KIND, int BN, bool PAIR>
 struct ProdShape {
   static constexpr int QR = PAIR ? BN / 2 : BN;                         // rows of Q that a CTA holds
   static constexpr int QCH = (BN + 127) / 128;                          // 128-row parts of Q
-  static constexpr int P_BYTES = PR_BM * 128, Q_BYTES = QR * 128, STAGE = HOLD ? Q_BYTES : P_BYTES + Q_BYTES;
+  static constexpr int P_BYTES = PR_BM * 128, Q_BYTES = QR * 128, STAGE = P_BYTES + Q_BYTES;
   // scales come in chunks of 4 words of 4 bytes a row (512 values): 2 (e2m1) or 4 (e4m3) stages
   static constexpr int CHUNK = KIND == 16 ? 0 : (1 + QCH) * 4 * 512, CHUNKS = 3, CHUNK_STAGES = KIND == 4 ? 2 : 4;
   static constexpr int SFC = KIND == 16 ? 0 : (1 + QCH) * 16;           // and their tensor-memory columns, two chunks in turn
-  static constexpr int FIXED = HOLD * P_BYTES + CHUNKS * CHUNK + 1024 + PR_STAGING + PR_GROUP_BYTES + 512;
+  static constexpr int FIXED = CHUNKS * CHUNK + 1024 + PR_STAGING + PR_GROUP_BYTES + 512;
   static constexpr int STAGES = (PR_SMEM_MAX - FIXED) / STAGE > 8 ? 8 : (PR_SMEM_MAX - FIXED) / STAGE;
   static constexpr int SMEM = STAGES * STAGE + FIXED;
   static constexpr int COLS = 2 * BN + 2 * SFC;
@@ -226,26 +221,23 @@ struct ProdTiles {
   const int *beg, *end, *cum;   // first row, row past the last, and first row tile of each group
   int n_groups, fixed;          // tiles of a row tile along the fixed axes
   int total, first, step;       // this CTA's (pair's) place among the `step` that walk the tiles
-  int lo, hi;                   // HOLD: its run of tiles
   // The r-th tile of this CTA (>= total: none).  DW's tiles are as long as their groups, the longest first
   // and every other round of them backwards, so that no CTA has the longest of every round.
-  template <int FORM, bool RUN>
+  template <int FORM>
   DEV int at(int r) const {
-    if (RUN) return lo + r < hi ? lo + r : total;   // neighbours, so that most have the same rows of P
     return r * step + (FORM == FORM_DW && (r & 1) ? step - 1 - first : first);
   }
 };
 
 struct ProdTile {
   int g, r0, r1;                // group, first row of the tile, row past the group's last
-  int f, u;                     // index along the fixed axes; row tile
+  int f;                        // index along the fixed axes
   DEV ProdTile uniform() const {
     ProdTile t;
     t.g = __shfl_sync(0xffffffffu, g, 0);
     t.r0 = __shfl_sync(0xffffffffu, r0, 0);
     t.r1 = __shfl_sync(0xffffffffu, r1, 0);
     t.f = __shfl_sync(0xffffffffu, f, 0);
-    t.u = __shfl_sync(0xffffffffu, u, 0);
     return t;
   }
 };
@@ -255,7 +247,6 @@ DEV ProdTile prod_tile(const ProdTiles& T, int t) {
   const int u = t / T.fixed;
   ProdTile r;
   r.f = t - u * T.fixed;
-  r.u = u;
   if (FORM == FORM_DW) {        // T.cum: the groups in order of length
     r.g = T.cum[u];
     r.r0 = T.beg[r.g];
@@ -274,11 +265,10 @@ DEV ProdTile prod_tile(const ProdTiles& T, int t) {
   return r;
 }
 
-template <int KIND, int BN, int FORM, bool PAIR, int HOLD>
+template <int KIND, int BN, int FORM, bool PAIR>
 __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
     k_prod(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ ProdArgs g) {
-  using S = ProdShape<KIND, BN, PAIR, HOLD>;
-  static_assert(!HOLD || (FORM == FORM_Y && !PAIR), "held rows: single CTAs, rows as P");
+  using S = ProdShape<KIND, BN, PAIR>;
   static_assert(!PAIR || (KIND == 16 && FORM != FORM_YT), "pairs: 16 bits, rows as P");
   constexpr int STAGES = S::STAGES;
   constexpr bool P_MN = FORM == FORM_DW, Q_MN = FORM == FORM_DX || FORM == FORM_DW;
@@ -289,7 +279,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   extern __shared__ unsigned char pr_raw[];
   unsigned char* base = (unsigned char*)(((uintptr_t)pr_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* sP = base;
-  unsigned char* sQ = sP + (HOLD ? HOLD : STAGES) * S::P_BYTES;
+  unsigned char* sQ = sP + STAGES * S::P_BYTES;
   unsigned char* sS = sQ + STAGES * S::Q_BYTES;
   unsigned char* staging = sS + S::CHUNKS * S::CHUNK;
   int* s_beg = (int*)(staging + PR_STAGING);
@@ -305,13 +295,15 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   uint64_t* tfull = cready + 2;
   uint64_t* tempty = tfull + 2;
   uint64_t* done = tempty + 2;
-  uint64_t* pfull = done + 1;            // HOLD: P's rows have landed, and the last MMA on them is done
-  uint64_t* pfree = pfull + 1;
-  uint32_t* tmem_slot = (uint32_t*)(pfree + 1);
+  uint32_t* tmem_slot = (uint32_t*)(done + 1);
   __shared__ int sh_fail;
   volatile int* failed = &sh_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
+  if (tid == 32) {   // the tensor maps are on their way while the rest is set up
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmB) : "memory");
+  }
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
       ag_mbar_init(&full[s], 1);
@@ -331,8 +323,6 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
       ag_mbar_init(&tempty[a], PR_EPI_WARPS * (PAIR ? 2 : 1));
     }
     ag_mbar_init(done, KIND == 16 ? 1 : 2);
-    ag_mbar_init(pfull, 1);
-    ag_mbar_init(pfree, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh_fail = 0;
   }
@@ -412,8 +402,6 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   T.total = __shfl_sync(0xffffffffu, *failed ? 0 : (FORM == FORM_DW ? g.n_groups : s_cum[g.n_groups]) * T.fixed, 0);
   T.first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
   T.step = PAIR ? gridDim.x >> 1 : gridDim.x;
-  T.lo = (int)((int64_t)T.total * T.first / T.step);
-  T.hi = (int)((int64_t)T.total * (T.first + 1) / T.step);
   const int red = FORM == FORM_DX ? g.n : g.k;   // (DW: the group's rows)
   bool ok = true;
 
@@ -424,20 +412,10 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   const auto wait = [](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, ag_wait(b, parity)) != 0; };
   if (warp == 0) {   // loads
     const bool one = pr_elect();
-    uint32_t it = 0, np = 0;
-    int held = -1;
-    for (int r = 0, t; (t = T.template at<FORM, (HOLD > 0)>(r)) < T.total && ok; ++r) {
+    uint32_t it = 0;
+    for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t).uniform();
       const int nk = ((FORM == FORM_DW ? c.r1 - c.r0 : red) + BK - 1) / BK;
-      if (HOLD && c.u != held) {
-        if (np >= 1 && !wait(pfree, (np - 1) & 1u)) { ok = false; break; }
-        if (one) {
-          ag_expect_tx(pfull, nk * S::P_BYTES);
-          for (int kb = 0; kb < nk; ++kb) ag_tma_2d(&tmA, pfull, sP + kb * S::P_BYTES, kb * 128, c.r0);
-        }
-        held = c.u;
-        ++np;
-      }
       for (int kb = 0; kb < nk; ++kb, ++it) {
         const int s = (int)(it % STAGES);
         if (it >= STAGES && !wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
@@ -446,7 +424,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
         ag_expect_tx(&full[s], S::STAGE);
         const int x = KIND == 16 ? kb * BK : kb * 128;   // microscaled rows are loaded as bytes
         if (FORM == FORM_Y) {
-          if (!HOLD) ag_tma_2d(&tmA, &full[s], p, x, c.r0 + rank * PR_BM);
+          ag_tma_2d(&tmA, &full[s], p, x, c.r0 + rank * PR_BM);
           pr_tma_3d(&tmB, &full[s], q, x, c.f * BN + rank * S::QR, c.g);
         } else if (FORM == FORM_YT) {
           pr_tma_3d(&tmB, &full[s], p, x, c.f * PR_BM, c.g);
@@ -465,24 +443,17 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
       }
     }
     // the last loads must have landed before the CTA ends
-    if (np) ok = wait(pfull, (np - 1) & 1u) && ok;
     for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j) ok = wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
     if (!ok) *failed = 1;
   } else if (warp == 1 && rank == 0) {   // MMAs
     const bool one = pr_elect();
-    uint32_t it = 0, j = 0, ci = 0, np = 0;
-    int held = -1;
+    uint32_t it = 0, j = 0, ci = 0;
     bool ready = false;
-    for (int t; (t = T.template at<FORM, (HOLD > 0)>(j)) < T.total && ok; ++j) {
+    for (int t; (t = T.template at<FORM>(j)) < T.total && ok; ++j) {
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t).uniform();
       const int len = FORM == FORM_DW ? c.r1 - c.r0 : red, nk = (len + BK - 1) / BK;
       const uint32_t acc = j & 1u;
       if (j >= 2 && !wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
-      if (HOLD && c.u != held) {
-        if (!wait(pfull, np & 1u)) { ok = false; break; }
-        held = c.u;
-        ++np;
-      }
       ag_fence_after();
       const uint32_t d = tmem + acc * BN;
       for (int kb = 0; kb < nk; ++kb, ++it) {
@@ -494,7 +465,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
         if (KIND != 16 && kb % S::CHUNK_STAGES == 0 && !wait(&cready[ci & 1u], (ci >> 1) & 1u)) { ok = false; break; }
         ready = pr_test(&landed[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u);   // the next stage, while this one's MMAs go out
         ag_fence_after();
-        const unsigned char *p = sP + (HOLD ? kb : s) * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
+        const unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
         const uint64_t dp = P_MN ? pr_desc_mn(p) : ag_desc(p), dq = Q_MN ? pr_desc_mn(q) : ag_desc(q);
         const int subs = left >= BK ? 4 : (left + SUB - 1) / SUB;
         if (one) {
@@ -519,10 +490,6 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
         }
         if (KIND != 16 && (kb % S::CHUNK_STAGES == S::CHUNK_STAGES - 1 || kb == nk - 1)) ++ci;
       }
-      if (HOLD) {
-        const int next = T.template at<FORM, (HOLD > 0)>(j + 1);
-        if (one && (next >= T.total || next / T.fixed != c.u)) ag_commit(pfree);
-      }
       if (one) pr_commit<PAIR>(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
     }
     if (one) ag_commit(done);   // every issued MMA has completed before the tensor memory is freed
@@ -531,7 +498,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
     const bool one = pr_elect();
     uint32_t ci = 0;
     const int chunks = (red + 511) / 512;
-    for (int r = 0, t; (t = T.template at<FORM, (HOLD > 0)>(r)) < T.total && ok; ++r) {
+    for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
       for (int i = 0; i < chunks; ++i, ++ci) {
         if (ci >= 2 && !wait(&cdone[ci & 1u], ((ci >> 1) & 1u) ^ 1u)) { ok = false; break; }
         if (!wait(&cfull[ci % S::CHUNKS], (ci / S::CHUNKS) & 1u)) { ok = false; break; }
@@ -553,7 +520,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
     if (KIND != 16 || (RELAY && warp - 2 < RELAYS)) {
       const int h = tid - 64;
       uint32_t it = 0;
-      for (int r = 0, t; (t = T.template at<FORM, (HOLD > 0)>(r)) < T.total && ok; ++r) {
+      for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
         const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
         if constexpr (KIND != 16) {
           // rows of w_g and rows of x, whichever is P
@@ -618,7 +585,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
     const int ew = warp - 4, quarter = ew & 3, half = ew >> 2;
     unsigned char* stg = staging + ew * 2048;
     uint32_t j = 0;
-    for (int t; (t = T.template at<FORM, (HOLD > 0)>(j)) < T.total; ++j) {
+    for (int t; (t = T.template at<FORM>(j)) < T.total; ++j) {
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
       const uint32_t acc = j & 1u;
       if (!__all_sync(0xffffffffu, pr_wait_long(&tfull[acc], (j >> 1) & 1u, failed) && !*failed)) {

@@ -61,9 +61,6 @@ static int encode(const char* who, CUtensorMap* m, const void* p, bool bytes, in
   return SMG_OK;
 }
 
-// Stages of a microscaled row that FORM_Y may hold (640 bytes: 1280 values of 4 bits); 4 stages are left for Q
-#define HELD 5
-
 // A product's operands: A has the packed rows, B the groups' fixed rows (DW: the packed rows of x)
 struct Operands {
   const void *a, *b;
@@ -71,9 +68,9 @@ struct Operands {
   int64_t a_len, b_len;   // values of a row (microscaled: bytes)
 };
 
-template <int KIND, int BN, int FORM, bool PAIR = false, int HOLD = 0>
+template <int KIND, int BN, int FORM, bool PAIR = false>
 static int launch(const char* who, const Operands& o, ProdArgs g, int type, cudaStream_t st) {
-  using S = ProdShape<KIND, BN, PAIR, HOLD>;
+  using S = ProdShape<KIND, BN, PAIR>;
   constexpr bool bytes = KIND != 16;
   const int wide = FORM == FORM_Y || FORM == FORM_YT ? g.n : g.k;
   const int pr = PAIR ? 2 * PR_BM : PR_BM;   // rows of P in a tile
@@ -104,7 +101,7 @@ static int launch(const char* who, const Operands& o, ProdArgs g, int type, cuda
   const int sms = sm_count(&dev);
   if (!sms) return fail(SMG_ERR_DEVICE, "%s: no usable device (%s)", who, cudaGetErrorString(cudaGetLastError()));
   if (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    const cudaError_t e = cudaFuncSetAttribute(k_prod<KIND, BN, FORM, PAIR, HOLD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(k_prod<KIND, BN, FORM, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return fail(SMG_ERR_DEVICE, "%s: %s", who, cudaGetErrorString(e));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
@@ -121,7 +118,7 @@ static int launch(const char* who, const Operands& o, ProdArgs g, int type, cuda
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = PAIR ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_prod<KIND, BN, FORM, PAIR, HOLD>, tA, tB, g);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_prod<KIND, BN, FORM, PAIR>, tA, tB, g);
   if (e != cudaSuccess) return fail(SMG_ERR_DEVICE, "%s: %s", who, cudaGetErrorString(e));
   return SMG_OK;
 }
@@ -269,8 +266,6 @@ int smg_mx_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_
     case 1: return bits == 4 ? launch<4, 64, FORM_YT>(who, o, g, 0, st) : launch<8, 64, FORM_YT>(who, o, g, 0, st);
     case 2: return bits == 4 ? launch<4, 128, FORM_YT>(who, o, g, 0, st) : launch<8, 128, FORM_YT>(who, o, g, 0, st);
   }
-  if (len <= HELD * 128 && (int64_t)rows * n >= 4ll * c.sms * PR_BM * 192)   // short rows, and tiles enough for runs
-    return bits == 4 ? launch<4, 192, FORM_Y, false, HELD>(who, o, g, 0, st) : launch<8, 192, FORM_Y, false, HELD>(who, o, g, 0, st);
   return bits == 4 ? launch<4, 192, FORM_Y>(who, o, g, 0, st) : launch<8, 192, FORM_Y>(who, o, g, 0, st);
 }
 

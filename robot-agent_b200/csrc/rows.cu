@@ -69,6 +69,8 @@ int smg_mx_values(const uint8_t* codes, const uint8_t* scales, int rows, int k, 
 // warps a row.  Rows off 16 bytes take the same shape, so that the order of the sums is the same.
 #define NORM_MAX_DIM 16384
 #define NORM_PARTS 296   // blocks of the gradient kernel, two an SM
+#define NORM_FEW 592     // rows (forward) for which a row of up to 2048 values gets a block's 8 warps: no more blocks than
+                         // the SMs hold at once, and a lane has one step instead of up to five in turn
 
 #define BY_STEPS5(steps, CALL)                     \
   do {                                             \
@@ -125,6 +127,11 @@ int smg_norm_add(const void* x, int64_t ldx, const void* r, int64_t ldr, const f
 #define CALL32(W, NV) LAUNCH(SMG_EMB_F32, W, NV)
 #define CALLBF(W, NV) LAUNCH(SMG_EMB_BF16, W, NV)
 #define CALLHF(W, NV) LAUNCH(SMG_EMB_F16, W, NV)
+  if (rows <= NORM_FEW && steps > 1 && steps <= 8) {
+    if (type == SMG_EMB_F32) { CALL32(8, 1); }
+    else if (type == SMG_EMB_BF16) { CALLBF(8, 1); }
+    else { CALLHF(8, 1); }
+  }
   if (type == SMG_EMB_F32) BY_STEPS3(steps, CALL32);
   else if (type == SMG_EMB_BF16) BY_STEPS5(steps, CALLBF);
   else BY_STEPS5(steps, CALLHF);

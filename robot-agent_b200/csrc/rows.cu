@@ -74,34 +74,34 @@ int smg_mx_values(const uint8_t* codes, const uint8_t* scales, int rows, int k, 
 
 #define BY_STEPS5(steps, CALL)                     \
   do {                                             \
-    if (steps <= 1) { CALL(1, 1); }     \
-    else if (steps <= 2) { CALL(1, 2); }     \
-    else if (steps <= 3) { CALL(1, 3); }     \
-    else if (steps <= 4) { CALL(1, 4); }     \
-    else if (steps <= 5) { CALL(1, 5); }     \
-    else if (steps <= 10) { CALL(2, 5); }    \
-    else if (steps <= 20) { CALL(4, 5); }    \
-    else if (steps <= 40) { CALL(8, 5); }    \
-    else { CALL(8, 8); }                     \
+    if (steps <= 1) { CALL(1, 1); }                \
+    else if (steps <= 2) { CALL(1, 2); }           \
+    else if (steps <= 3) { CALL(1, 3); }           \
+    else if (steps <= 4) { CALL(1, 4); }           \
+    else if (steps <= 5) { CALL(1, 5); }           \
+    else if (steps <= 10) { CALL(2, 5); }          \
+    else if (steps <= 20) { CALL(4, 5); }          \
+    else if (steps <= 40) { CALL(8, 5); }          \
+    else { CALL(8, 8); }                           \
   } while (0)
 #define BY_STEPS3(steps, CALL)                     \
   do {                                             \
-    if (steps <= 1) { CALL(1, 1); }     \
-    else if (steps <= 2) { CALL(1, 2); }     \
-    else if (steps <= 3) { CALL(1, 3); }     \
-    else if (steps <= 6) { CALL(2, 3); }     \
-    else if (steps <= 12) { CALL(4, 3); }    \
-    else if (steps <= 24) { CALL(8, 3); }    \
-    else { CALL(8, 8); }                     \
+    if (steps <= 1) { CALL(1, 1); }                \
+    else if (steps <= 2) { CALL(1, 2); }           \
+    else if (steps <= 3) { CALL(1, 3); }           \
+    else if (steps <= 6) { CALL(2, 3); }           \
+    else if (steps <= 12) { CALL(4, 3); }          \
+    else if (steps <= 24) { CALL(8, 3); }          \
+    else { CALL(8, 8); }                           \
   } while (0)
 #define BY_STEPS2(steps, CALL)                     \
   do {                                             \
-    if (steps <= 1) { CALL(1, 1); }     \
-    else if (steps <= 2) { CALL(1, 2); }     \
-    else if (steps <= 4) { CALL(2, 2); }     \
-    else if (steps <= 8) { CALL(4, 2); }     \
-    else if (steps <= 16) { CALL(8, 2); }    \
-    else { CALL(8, 8); }                     \
+    if (steps <= 1) { CALL(1, 1); }                \
+    else if (steps <= 2) { CALL(1, 2); }           \
+    else if (steps <= 4) { CALL(2, 2); }           \
+    else if (steps <= 8) { CALL(4, 2); }           \
+    else if (steps <= 16) { CALL(8, 2); }          \
+    else { CALL(8, 8); }                           \
   } while (0)
 
 int smg_norm_add(const void* x, int64_t ldx, const void* r, int64_t ldr, const float* gain, int rows, int dim, int type, float eps,

@@ -51,7 +51,7 @@ struct Elem<SMG_EMB_F16> {
 template <int TYPE>
 struct Raw8 {
   typedef typename Elem<TYPE>::T T;
-  union { uint4 q[sizeof(T) / 2]; T t[8]; };
+  union { uint4 q[sizeof(T) / 2]; T t[8]; uint32_t w[2 * sizeof(T)]; };
   template <bool VEC>
   DEV void load(const T* p, int n) {   // p is used only where n > 0
     if constexpr (VEC) {
@@ -64,6 +64,57 @@ struct Raw8 {
   }
   DEV float get(int i) const { return Elem<TYPE>::up(t[i]); }
 };
+
+// N words of w + `bytes` (0 .. 15): w has N + 4
+template <int N>
+DEV void words_from(const uint32_t (&w)[N + 4], uint32_t bytes, uint32_t (&out)[N]) {
+  uint32_t a[N + 2], b[N + 1];
+#pragma unroll
+  for (int i = 0; i < N + 2; ++i) a[i] = bytes & 8u ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < N + 1; ++i) b[i] = bytes & 4u ? a[i + 1] : a[i];
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(b[i], b[i + 1], (bytes & 3u) * 8);
+}
+
+// The same of rows that start anywhere (a matrix of odd length): the 16-byte words around the 8 values, as far
+// as they lie within the matrix (lo .. hi), then a shift; value by value at its two ends.
+template <int TYPE>
+struct Any8 {
+  typedef typename Elem<TYPE>::T T;
+  static constexpr int V = sizeof(T) / 2;   // 16-byte words of 8 values
+  uint32_t w[4 * V + 4];
+  const T* p;
+  int n;
+  bool in;
+  DEV void begin(const T* at, int left, uintptr_t lo, uintptr_t hi) {
+    p = at;
+    n = left;
+    const uintptr_t a = (uintptr_t)at & ~(uintptr_t)15;
+    in = n > 0 && a >= lo && a + 16 * (V + 1) <= hi;
+#pragma unroll
+    for (int i = 0; i <= V; ++i) {
+      const uint4 q = in ? __ldg((const uint4*)a + i) : make_uint4(0, 0, 0, 0);
+      w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+    }
+  }
+  DEV void end(Raw8<TYPE>& r) const {
+    if (in) {
+      words_from<4 * V>(w, (uint32_t)((uintptr_t)p & 15), r.w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= n) r.t[i] = Elem<TYPE>::down(0.f);
+    } else {
+      r.template load<false>(p, n);
+    }
+  }
+};
+
+// One past the last byte of a matrix
+template <typename T>
+DEV uintptr_t rows_end(const void* p, int64_t rows, int64_t ld, int dim) {
+  return (uintptr_t)p + ((rows - 1) * ld + dim) * sizeof(T);
+}
 
 template <int TYPE>
 DEV void store8(typename Elem<TYPE>::T* p, int n, bool vec, const float (&v)[8]) {
@@ -83,6 +134,36 @@ DEV void store8(typename Elem<TYPE>::T* p, int n, bool vec, const float (&v)[8])
 
 // 2^e, -127 <= e <= 127
 DEV float mx_two(int e) { return __int_as_float(e > -127 ? (e + 127) << 23 : 1 << 22); }
+
+// 8 16-bit values (as 4 words) to p, n of them there; the lanes' places j count along a row, and all 32 lanes
+// call this together.  Off 16 bytes a lane stores the aligned 16 bytes that begin in its values and end in its
+// neighbour's; what no such store takes (the ends of a row and of the warp) goes value by value.
+DEV void store8_any(uint16_t* p, int n, int j, const uint32_t (&c)[4]) {
+  const uint32_t sh = (uint32_t)(uintptr_t)p & 15u, lane = threadIdx.x & 31;
+  uint32_t w[8], out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = c[i];
+    w[4 + i] = __shfl_down_sync(0xffffffffu, c[i], 1);
+  }
+  const int nj = __shfl_down_sync(0xffffffffu, j, 1), nn = __shfl_down_sync(0xffffffffu, n, 1), pj = __shfl_up_sync(0xffffffffu, j, 1);
+  if (n <= 0) return;
+  if (sh == 0 && n >= 8) {
+    *(uint4*)p = make_uint4(c[0], c[1], c[2], c[3]);
+    return;
+  }
+  const int head = (int)(16 - sh) / 2;   // values before the aligned 16 bytes
+  const bool mine = sh && lane < 31 && nj == j + 1 && nn >= head && n >= 8;
+  const bool before = sh && lane > 0 && pj == j - 1 && n >= head;   // the neighbour's store takes my first ones
+  if (mine) {
+    words_from<4>(w, 16 - sh, out);
+    *(uint4*)(p + head) = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+  const int from = before ? head : 0, to = mine ? head : n < 8 ? n : 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i >= from && i < to) p[i] = (uint16_t)(c[i >> 1] >> (16 * (i & 1)));
+}
 
 DEV float max_nan(float a, float b) {
   float r;
@@ -202,32 +283,29 @@ DEV void mx_emit(const MxOut& o, int64_t row, int j, const float (&v)[8]) {
   m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const int b = j >> 2;
-  if (b >= o.pitch) return;
+  const bool there = b < o.kb;
   const uint32_t s = mx_scale<BITS>(m);
-  if (o.scales && !(j & 3)) o.scales[row * o.pitch + b] = (uint8_t)(b < o.kb ? s : 0u);
-  if (b >= o.kb) return;
+  if (o.scales && !(j & 3) && b < o.pitch) o.scales[row * o.pitch + b] = (uint8_t)(there ? s : 0u);
   const float inv = __uint_as_float(s == 255u ? 0x3f800000u : (254u - s) << 23);
   float u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) u[i] = v[i] * inv;
   uint32_t c[2];
   mx_codes<BITS>(u, c);
-  if (o.codes) {
+  if (o.codes && there) {
     uint8_t* d = o.codes + (row * o.kb * 4 + j) * BITS;   // 8 values are BITS bytes
     if (BITS == 4) *(uint32_t*)d = c[0];
     else *(uint2*)d = make_uint2(c[0], c[1]);
   }
   if (o.values) {
-    union { uint32_t w[4]; uint16_t h[8]; } q;
-    mx_values8<BITS>(c, s, q.w);
-    __nv_bfloat16* d = o.values + row * o.dim + 8 * j;
+    uint32_t q[4];
+    mx_values8<BITS>(c, s, q);
+    uint16_t* d = (uint16_t*)o.values + row * o.dim + 8 * j;
     const int n = o.dim - 8 * j;
     if (!(o.dim & 7)) {
-      if (n > 0) *(uint4*)d = make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
+      if (n > 0) *(uint4*)d = make_uint4(q[0], q[1], q[2], q[3]);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) ((uint16_t*)d)[i] = q.h[i];
+      store8_any(d, n, j, q);
     }
   }
 }
@@ -248,19 +326,27 @@ DEV void mx_place(int64_t t, int64_t n, const MxDiv& d, int64_t& row, int& j) {
 // it reads the input once and writes bits / 8 + 1/32 bytes (and 2 with `values`).
 #define MX_EACH 4
 template <int TYPE, int BITS, bool VEC>
-__global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::T* x, int64_t ldx, int64_t n, MxDiv div, MxOut o) {
+__global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::T* x, int64_t ldx, int rows, int64_t n, MxDiv div, MxOut o) {
   heads_next();
   heads_wait();
   const int64_t t0 = (int64_t)blockIdx.x * (256 * MX_EACH) + threadIdx.x;
   Raw8<TYPE> raw[MX_EACH];
+  Any8<TYPE> any[VEC ? 1 : MX_EACH];
   int64_t row[MX_EACH];
   int j[MX_EACH];
+  const uintptr_t hi = rows_end<typename Elem<TYPE>::T>(x, rows, ldx, o.dim);
 #pragma unroll
   for (int i = 0; i < MX_EACH; ++i) {
     mx_place(t0 + i * 256, n, div, row[i], j[i]);
     // n and a row's parts are multiples of 4, so the lanes of a block of 32 are all in or all out of range
     if (t0 + i * 256 >= n) { row[i] = 0; j[i] = o.pitch * 4; }
-    raw[i].template load<VEC>(x + row[i] * ldx + 8 * j[i], o.dim - 8 * j[i]);
+    const typename Elem<TYPE>::T* p = x + row[i] * ldx + 8 * j[i];
+    if constexpr (VEC) raw[i].template load<true>(p, o.dim - 8 * j[i]);
+    else any[i].begin(p, o.dim - 8 * j[i], (uintptr_t)x, hi);
+  }
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < MX_EACH; ++i) any[i].end(raw[i]);
   }
 #pragma unroll
   for (int i = 0; i < MX_EACH; ++i) {

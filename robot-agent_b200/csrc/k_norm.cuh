@@ -42,6 +42,50 @@ DEV float row_sum(float v, float* scr, int sub) {
   return v;
 }
 
+// a lane's values of `row` of two matrices, all loads first (a null matrix gives zeros)
+template <int TYPE, int WARPS, int NV, bool VEC>
+DEV void row_load2(Raw8<TYPE> (&q)[NV], const void* p, int64_t ldp, Raw8<TYPE> (&u)[NV], const void* o, int64_t ldo, int64_t row, int t,
+                   const NormArgs& a) {
+  typedef typename Elem<TYPE>::T T;
+  const T *ap = (const T*)p + (p ? row * ldp : 0), *ao = (const T*)o + (o ? row * ldo : 0);
+  const int dp = p ? a.dim : 0, dn = o ? a.dim : 0;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (t + i * 32 * WARPS);
+      q[i].template load<true>(ap + c, dp - c);
+      u[i].template load<true>(ao + c, dn - c);
+    }
+  } else {
+    const uintptr_t hp = rows_end<T>(p, a.rows, ldp, a.dim), ho = rows_end<T>(o, a.rows, ldo, a.dim);
+    Any8<TYPE> w[NV], v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (t + i * 32 * WARPS);
+      w[i].begin(ap + c, dp - c, (uintptr_t)p, hp);
+      v[i].begin(ao + c, dn - c, (uintptr_t)o, ho);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      w[i].end(q[i]);
+      v[i].end(u[i]);
+    }
+  }
+}
+
+// 8 values at c of a row; all lanes of the warp together
+template <int TYPE, bool VEC>
+DEV void row_store(typename Elem<TYPE>::T* p, int c, int dim, const float (&v)[8]) {
+  if constexpr (VEC || TYPE == SMG_EMB_F32) {
+    store8<TYPE>(p + c, dim - c, VEC, v);
+  } else {
+    Raw8<TYPE> q;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q.t[i] = Elem<TYPE>::down(v[i]);
+    store8_any((uint16_t*)(p + c), dim - c, c >> 3, q.w);
+  }
+}
+
 // 1 / sqrt(ss / dim + eps) as a float and what it lacks (both together good to about 2^-45): the float's
 // residual 1 - (v + ve) r^2, with v + ve the argument before its roundings, halved, corrects it (one Newton step).
 DEV float rstd_of(float ss, float dim, float eps, float& low) {
@@ -53,11 +97,12 @@ DEV float rstd_of(float ss, float dim, float eps, float& low) {
   return r;
 }
 
-// gain of 8 columns; VEC: on 16 bytes, n a multiple of 8
+// gain of 8 columns (VEC: on 16 bytes and n a multiple of 8)
 template <bool VEC>
 DEV void gain8(const float* p, int n, float (&g)[8]) {
   Raw8<SMG_EMB_F32> q;
-  q.template load<VEC>(p, n);
+  if (VEC || (n >= 8 && !((uintptr_t)p & 15))) q.template load<true>(p, n);
+  else q.template load<false>(p, n);
 #pragma unroll
   for (int i = 0; i < 8; ++i) g[i] = q.get(i);
 }
@@ -74,18 +119,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_add(NormArgs a) {
   float h[NV][8];
   {
     Raw8<TYPE> x[NV], r[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (t + i * 32 * WARPS);
-      x[i].template load<VEC>((const T*)a.x + row * a.ldx + c, a.dim - c);
-    }
-    if (a.r) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = 8 * (t + i * 32 * WARPS);
-        r[i].template load<VEC>((const T*)a.r + row * a.ldr + c, a.dim - c);
-      }
-    }
+    row_load2<TYPE, WARPS, NV, VEC>(x, a.x, a.ldx, r, a.r, a.ldr, row, t, a);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -107,7 +141,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_add(NormArgs a) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = t + i * 32 * WARPS, c = 8 * j, n = a.dim - c;
-    if (a.h) store8<TYPE>((T*)a.h + row * a.ldh + c, n, VEC, h[i]);
+    if (a.h) row_store<TYPE, VEC>((T*)a.h + row * a.ldh, c, a.dim, h[i]);
     float g[8];
     gain8<VEC>(a.gain + c, n, g);
 #pragma unroll
@@ -135,14 +169,8 @@ __global__ void __launch_bounds__(NORM_THREADS, NV <= 3 ? 2 : 1) k_norm_add_bwd(
   const int64_t step = (int64_t)gridDim.x * NORM_ROWS(WARPS);
   for (int64_t row = (int64_t)blockIdx.x * NORM_ROWS(WARPS) + sub; row < a.rows; row += step) {
     Raw8<TYPE> x[NV], r[NV], y[NV], d[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (t + i * 32 * WARPS);
-      x[i].template load<VEC>((const T*)a.x + row * a.ldx + c, a.dim - c);
-      y[i].template load<VEC>((const T*)a.dy + row * a.ldy + c, a.dim - c);
-      r[i].template load<VEC>((const T*)a.r + row * a.ldr + c, a.r ? a.dim - c : 0);
-      d[i].template load<VEC>((const T*)a.dh + row * a.ldh_in + c, a.dh ? a.dim - c : 0);
-    }
+    row_load2<TYPE, WARPS, NV, VEC>(x, a.x, a.ldx, y, a.dy, a.ldy, row, t, a);
+    row_load2<TYPE, WARPS, NV, VEC>(r, a.r, a.ldr, d, a.dh, a.ldh_in, row, t, a);
     const float rstd = a.rstd[row];
     float dot = 0.f;
 #pragma unroll
@@ -168,7 +196,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NV <= 3 ? 2 : 1) k_norm_add_bwd(
         const float n = (x[i].get(k) + r[i].get(k)) * rstd;
         o[k] = __fmaf_rn(rstd, __fmaf_rn(-n, dot, y[i].get(k) * g[k]), d[i].get(k));
       }
-      store8<TYPE>((T*)a.dx + row * a.lddx + c, a.dim - c, VEC, o);
+      row_store<TYPE, VEC>((T*)a.dx + row * a.lddx, c, a.dim, o);
     }
   }
   float* part = a.part + (int64_t)blockIdx.x * a.dim;

@@ -37,7 +37,7 @@ int smg_mx_quantise(const void* x, int64_t ldx, int rows, int k, int type, int b
 #define CALL(TY)                                                                                              \
   const auto f = bits == 4 ? (vec ? k_mx_quantise<TY, 4, true> : k_mx_quantise<TY, 4, false>)                 \
                            : (vec ? k_mx_quantise<TY, 8, true> : k_mx_quantise<TY, 8, false>);                \
-  return launch_next(who, f, grid, 256, 0, st, (const Elem<TY>::T*)x, ldx, n, mx_div(o.pitch * 4), o)
+  return launch_next(who, f, grid, 256, 0, st, (const Elem<TY>::T*)x, ldx, rows, n, mx_div(o.pitch * 4), o)
   BY_TYPE(type, CALL);
 #undef CALL
 }

@@ -409,6 +409,10 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   // the compiler can see to be the warp's (votes, values handed on by a shuffle): their operands live in
   // uniform registers.  From a single thread's own code each MMA took 115 cycles to issue whatever its
   // width, a block-scaled one with branches on values out of shared memory 220 (32 to 128 are needed).
+  // A pair's last tile with no more than half of its columns: MMAs of half the width
+  const auto slim = [&](const ProdTile& c) {
+    return PAIR && (FORM == FORM_Y ? g.n : g.k) - (FORM == FORM_DW ? c.f / g.p_tiles : c.f) * BN <= BN / 2;
+  };
   const auto wait = [](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, ag_wait(b, parity)) != 0; };
   if (warp == 0) {   // loads
     const bool one = pr_elect();
@@ -416,6 +420,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
     for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t).uniform();
       const int nk = ((FORM == FORM_DW ? c.r1 - c.r0 : red) + BK - 1) / BK;
+      const int half = rank * (slim(c) ? S::QR / 2 : S::QR);   // where this CTA's part of Q begins
       for (int kb = 0; kb < nk; ++kb, ++it) {
         const int s = (int)(it % STAGES);
         if (it >= STAGES && !wait(&empty[s], ((it / STAGES) & 1u) ^ 1u)) { ok = false; break; }
@@ -425,16 +430,16 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
         const int x = KIND == 16 ? kb * BK : kb * 128;   // microscaled rows are loaded as bytes
         if (FORM == FORM_Y) {
           ag_tma_2d(&tmA, &full[s], p, x, c.r0 + rank * PR_BM);
-          pr_tma_3d(&tmB, &full[s], q, x, c.f * BN + rank * S::QR, c.g);
+          pr_tma_3d(&tmB, &full[s], q, x, c.f * BN + half, c.g);
         } else if (FORM == FORM_YT) {
           pr_tma_3d(&tmB, &full[s], p, x, c.f * PR_BM, c.g);
           ag_tma_2d(&tmA, &full[s], q, x, c.r0);
         } else if (FORM == FORM_DX) {
           ag_tma_2d(&tmA, &full[s], p, x, c.r0 + rank * PR_BM);
 #pragma unroll
-          for (int j = 0; j < S::QR / 64; ++j) pr_tma_3d(&tmB, &full[s], q + j * 8192, c.f * BN + rank * S::QR + j * 64, x, c.g);
+          for (int j = 0; j < S::QR / 64; ++j) pr_tma_3d(&tmB, &full[s], q + j * 8192, c.f * BN + half + j * 64, x, c.g);
         } else {
-          const int m0 = c.f % g.p_tiles * RT + rank * PR_BM, n0 = c.f / g.p_tiles * BN + rank * S::QR;
+          const int m0 = c.f % g.p_tiles * RT + rank * PR_BM, n0 = c.f / g.p_tiles * BN + half;
 #pragma unroll
           for (int j = 0; j < PR_BM / 64; ++j) ag_tma_2d(&tmA, &full[s], p + j * 8192, m0 + j * 64, c.r0 + x);
 #pragma unroll
@@ -456,6 +461,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
       if (j >= 2 && !wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
       ag_fence_after();
       const uint32_t d = tmem + acc * BN;
+      const uint32_t idesc = slim(c) ? (g.idesc & ~(0x3fu << 17)) | (uint32_t)(BN / 16) << 17 : g.idesc;
       for (int kb = 0; kb < nk; ++kb, ++it) {
         const int s = (int)(it % STAGES);
         const uint32_t ph = (it / STAGES) & 1u;
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
           if constexpr (KIND == 16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (i < subs) pr_mma16<PAIR>(d, dp + i * (P_MN ? 128 : 2), dq + i * (Q_MN ? 128 : 2), g.idesc, (kb | i) != 0);
+              if (i < subs) pr_mma16<PAIR>(d, dp + i * (P_MN ? 128 : 2), dq + i * (Q_MN ? 128 : 2), idesc, (kb | i) != 0);
           } else {
             const uint32_t tp = tmem + 2 * BN + (ci & 1u) * S::SFC, tq = tp + 16;
             const uint32_t w0 = KIND == 4 ? kb % 2 * 2 : kb % 4;   // the stage's first word of the chunk
@@ -481,7 +487,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
               if (i < subs) {
                 // an MMA's 2 scales of a row (e2m1) are half a word, its one (e4m3) is a byte of it
                 const uint32_t w = w0 + (KIND == 4 ? i / 2 : 0), id = KIND == 4 ? (i & 1) * 2 : i;
-                pr_mma_mx<KIND>(d, dp + i * 2, dq + i * 2, g.idesc | id << 29 | id << 4, tp + 4 * w, tq + 4 * S::QCH * w, (kb | i) != 0);
+                pr_mma_mx<KIND>(d, dp + i * 2, dq + i * 2, idesc | id << 29 | id << 4, tp + 4 * w, tq + 4 * S::QCH * w, (kb | i) != 0);
               }
             }
             if (kb % S::CHUNK_STAGES == S::CHUNK_STAGES - 1 || kb == nk - 1) ag_commit(&cdone[ci & 1u]);

@@ -27,7 +27,7 @@
 //               wants (row r of 128 at 16 (r % 32) + 4 (r / 32) of 512 bytes for each 4 blocks).  DW: zeros over the
 //               rows past the group's end in its last block, where the load brought the next group's
 //               rows (in both operands, since zero times NaN is NaN), reported on fixed[s];
-//               Pairs: they pass a landed stage on to the leader's fixed[s];
+//               Pairs: warp 2 (microscaled rows: warp 13) passes a landed stage on to the leader's fixed[s];
 //   warp 12     (microscaled rows) copies landed scales to tensor memory, two chunks in turn (cready / cdone): in
 //               the MMA warp the copies and their waits took 300 cycles of the 384 that a stage has;
 //   warps 4-11  read D from tensor memory, round once and store.  Rows past the group's end and
@@ -36,7 +36,8 @@
 // of P and one half of Q and keeps the sums of its rows; rank 0 issues the MMAs of both, which read
 // each half of Q once for the two.  That is what the single form lacks: at 128 x 256 a CTA writes 48 KB into
 // shared memory and reads 48 KB out of it for 512 cycles of MMAs, 192 bytes a cycle where an SM has 128;
-// in a pair it is 32 + 32 KB.
+// in a pair it is 32 + 32 KB (microscaled rows,
+// 128 x 192: 40 + 40 KB for 384 cycles, in a pair 28 + 28).
 //
 // Every wait is bounded, or goes on only until another role's bounded wait has run out; then the
 // roles run out too, SMG_PROD_TIMEOUT is set, and the CTA waits (bounded) for its own copies and
@@ -62,7 +63,7 @@ struct ProdArgs {
 };
 
 #define PR_BM 128
-#define PR_THREADS(KIND) (KIND == 16 ? 384 : 416)
+#define PR_THREADS(KIND, PAIR) (KIND == 16 ? 384 : PAIR ? 448 : 416)
 #define PR_HELPERS 64
 #define PR_EPI_WARPS 8
 #define PR_SMEM_MAX 232448
@@ -124,24 +125,28 @@ DEV void pr_mma16(uint32_t d, uint64_t p, uint64_t q, uint32_t idesc, uint32_t a
         "l"(p), "l"(q), "r"(idesc), "r"(accum));
 }
 
-template <int KIND>
+template <int KIND, bool PAIR>
 DEV void pr_mma_mx(uint32_t d, uint64_t p, uint64_t q, uint32_t idesc, uint32_t sp, uint32_t sq, uint32_t accum) {
-  if constexpr (KIND == 4)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-        "l"(p), "l"(q), "r"(idesc), "r"(sp), "r"(sq), "r"(accum));
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-        "l"(p), "l"(q), "r"(idesc), "r"(sp), "r"(sq), "r"(accum));
+#define PR_MMA_MX(GROUP, WHAT)                                                                                         \
+  asm volatile(                                                                                                        \
+      "{\n\t.reg .pred p;\n\t"                                                                                        \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                                     \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" WHAT " [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),             \
+      "l"(p), "l"(q), "r"(idesc), "r"(sp), "r"(sq), "r"(accum))
+  if constexpr (KIND == 4 && PAIR) PR_MMA_MX("2", "mxf4.block_scale.scale_vec::2X");
+  else if constexpr (KIND == 4) PR_MMA_MX("1", "mxf4.block_scale.scale_vec::2X");
+  else if constexpr (PAIR) PR_MMA_MX("2", "mxf8f6f4.block_scale.scale_vec::1X");
+  else PR_MMA_MX("1", "mxf8f6f4.block_scale.scale_vec::1X");
+#undef PR_MMA_MX
 }
 
+// 512 bytes of scales to tensor memory (PAIR: of each CTA to its own)
+template <bool PAIR>
 DEV void pr_copy_scales(uint32_t tmem, const void* p) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(pr_desc_scales(p)) : "memory");
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(pr_desc_scales(p)) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(pr_desc_scales(p)) : "memory");
 }
 
 // true in one lane of a converged warp
@@ -266,16 +271,16 @@ DEV ProdTile prod_tile(const ProdTiles& T, int t) {
 }
 
 template <int KIND, int BN, int FORM, bool PAIR>
-__global__ void __launch_bounds__(PR_THREADS(KIND), 1)
+__global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
     k_prod(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ ProdArgs g) {
   using S = ProdShape<KIND, BN, PAIR>;
-  static_assert(!PAIR || (KIND == 16 && FORM != FORM_YT), "pairs: 16 bits, rows as P");
+  static_assert(!PAIR || FORM != FORM_YT, "pairs: rows as P");
   constexpr int STAGES = S::STAGES;
   constexpr bool P_MN = FORM == FORM_DW, Q_MN = FORM == FORM_DX || FORM == FORM_DW;
   constexpr int BK = P_MN || Q_MN ? 64 : 1024 / KIND;   // values of the reduction axis in a stage
   constexpr int SUB = BK / 4;                           // and in an MMA
-  constexpr bool RELAY = PAIR || FORM == FORM_DW;       // warps 2, 3 pass every stage on
-  constexpr int RELAYS = FORM == FORM_DW ? PR_HELPERS / 32 : 1;
+  constexpr bool RELAY = PAIR || FORM == FORM_DW;       // every landed stage is passed on
+  constexpr int RELAYS = FORM == FORM_DW ? PR_HELPERS / 32 : 1, RELAY_WARP = KIND == 16 ? 2 : 13;   // by so many warps from this one
   extern __shared__ unsigned char pr_raw[];
   unsigned char* base = (unsigned char*)(((uintptr_t)pr_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* sP = base;
@@ -292,7 +297,8 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   uint64_t* cempty = cfull + S::CHUNKS;  // has been copied to tensor memory,
   uint64_t* cdone = cempty + S::CHUNKS;  // and the MMAs that use the copy are done
   uint64_t* cready = cdone + 2;          // the copy is in tensor memory
-  uint64_t* tfull = cready + 2;
+  uint64_t* cpeer = cready + 2;          // PAIR: the other CTA's chunk has landed
+  uint64_t* tfull = cpeer + S::CHUNKS;
   uint64_t* tempty = tfull + 2;
   uint64_t* done = tempty + 2;
   uint32_t* tmem_slot = (uint32_t*)(done + 1);
@@ -313,6 +319,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
     for (int s = 0; s < S::CHUNKS; ++s) {
       ag_mbar_init(&cfull[s], PR_HELPERS);
       ag_mbar_init(&cempty[s], 1);
+      ag_mbar_init(&cpeer[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       ag_mbar_init(&cdone[a], 1);
@@ -343,7 +350,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   heads_wait();   // barriers and tensor memory are set up; from here on global memory is read
   // groups: offsets that break the rules are reported, and every group is then taken as empty
   int bad = 0;
-  for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND)) {
+  for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND, PAIR)) {
     int a = 0, b = g.rows;
     if (g.off) {
       a = g.off[i];
@@ -358,7 +365,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   ag_fence_after();
   if (bad) {
     if (tid == 0 && blockIdx.x == 0 && g.err) atomicOr(g.err, SMG_PROD_OFFSETS);
-    for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND)) s_beg[i] = s_end[i] = 0;
+    for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND, PAIR)) s_beg[i] = s_end[i] = 0;
     __syncthreads();
   }
   constexpr uint32_t tmem = 0;
@@ -366,7 +373,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
   constexpr int RT = FORM == FORM_YT ? BN : PAIR ? 2 * PR_BM : PR_BM;
   const int rank = PAIR ? (int)pr_rank() : 0;   // which of a pair's 128 rows of P (and halves of Q) are this CTA's
   if (FORM == FORM_DW) {   // groups by length (beyond 256 of them, where no single one holds the end up, as they come)
-    for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND)) {
+    for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND, PAIR)) {
       int rank = i;
       if (g.n_groups <= 256) {
         const int len = s_end[i] - s_beg[i];
@@ -487,10 +494,10 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
               if (i < subs) {
                 // an MMA's 2 scales of a row (e2m1) are half a word, its one (e4m3) is a byte of it
                 const uint32_t w = w0 + (KIND == 4 ? i / 2 : 0), id = KIND == 4 ? (i & 1) * 2 : i;
-                pr_mma_mx<KIND>(d, dp + i * 2, dq + i * 2, idesc | id << 29 | id << 4, tp + 4 * w, tq + 4 * S::QCH * w, (kb | i) != 0);
+                pr_mma_mx<KIND, PAIR>(d, dp + i * 2, dq + i * 2, idesc | id << 29 | id << 4, tp + 4 * w, tq + 4 * S::QCH * w, (kb | i) != 0);
               }
             }
-            if (kb % S::CHUNK_STAGES == S::CHUNK_STAGES - 1 || kb == nk - 1) ag_commit(&cdone[ci & 1u]);
+            if (kb % S::CHUNK_STAGES == S::CHUNK_STAGES - 1 || kb == nk - 1) pr_commit<PAIR>(&cdone[ci & 1u]);
           }
           pr_commit<PAIR>(&empty[s]);
         }
@@ -498,7 +505,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
       }
       if (one) pr_commit<PAIR>(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
     }
-    if (one) ag_commit(done);   // every issued MMA has completed before the tensor memory is freed
+    if (one) pr_commit<PAIR>(done);   // every issued MMA has completed before the tensor memory is freed
     if (!wait(done, 0) || !ok) *failed = 1;
   } else if (warp == 12) {   // microscaled rows: scales from shared to tensor memory
     const bool one = pr_elect();
@@ -506,87 +513,95 @@ __global__ void __launch_bounds__(PR_THREADS(KIND), 1)
     const int chunks = (red + 511) / 512;
     for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
       for (int i = 0; i < chunks; ++i, ++ci) {
-        if (ci >= 2 && !wait(&cdone[ci & 1u], ((ci >> 1) & 1u) ^ 1u)) { ok = false; break; }
-        if (!wait(&cfull[ci % S::CHUNKS], (ci / S::CHUNKS) & 1u)) { ok = false; break; }
+        const uint32_t s = ci % S::CHUNKS, ph = (ci / S::CHUNKS) & 1u;
+        if (rank == 0 && ci >= 2 && !wait(&cdone[ci & 1u], ((ci >> 1) & 1u) ^ 1u)) { ok = false; break; }
+        if (!wait(&cfull[s], ph)) { ok = false; break; }
         pr_proxy_fence();   // they were written by ordinary copies
+        if (PAIR && rank == 1) {
+          if (one) pr_arrive_leader(&cpeer[s]);
+          continue;
+        }
+        if (PAIR && !wait(&cpeer[s], ph)) { ok = false; break; }
         ag_fence_after();
         if (one) {
-          const unsigned char* sc = sS + ci % S::CHUNKS * S::CHUNK;
+          const unsigned char* sc = sS + s * S::CHUNK;
           const uint32_t tp = tmem + 2 * BN + (ci & 1u) * S::SFC;
 #pragma unroll
-          for (int k = 0; k < 4 * (1 + S::QCH); ++k) pr_copy_scales(tp + 4 * k, sc + 512 * k);
-          ag_commit(&cempty[ci % S::CHUNKS]);
-          ag_commit(&cready[ci & 1u]);
+          for (int k = 0; k < 4 * (1 + S::QCH); ++k) pr_copy_scales<PAIR>(tp + 4 * k, sc + 512 * k);
+          pr_commit<PAIR>(&cempty[s]);
+          pr_commit<PAIR>(&cready[ci & 1u]);
         }
       }
     }
-    if (one) ag_commit(done);
+    if (one && rank == 0) pr_commit<PAIR>(done);
     if (!ok) *failed = 1;
-  } else if (warp == 2 || warp == 3) {
-    if (KIND != 16 || (RELAY && warp - 2 < RELAYS)) {
-      const int h = tid - 64;
-      uint32_t it = 0;
-      for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
-        const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
-        if constexpr (KIND != 16) {
-          // rows of w_g and rows of x, whichever is P
-          const int w0 = c.f * (FORM == FORM_YT ? PR_BM : BN);
-          const int p_lim = FORM == FORM_YT ? g.n - w0 : c.r1 - c.r0, q_lim = FORM == FORM_YT ? c.r1 - c.r0 : g.n - w0;
-          const int64_t wr = (int64_t)c.g * g.n + w0, xr = c.r0;
-          const uint8_t* ps = (FORM == FORM_YT ? g.sb + wr * g.pitch : g.sa + xr * g.pitch);
-          const uint8_t* qs = (FORM == FORM_YT ? g.sa + xr * g.pitch : g.sb + wr * g.pitch);
-          // 8 rows x 16 bytes a warp and step: thread h has word h % 4 of the rows h / 4, h / 4 + 16, ...
-          const int r0 = h >> 2, w = h & 3;
-          for (int k0 = 0; k0 < g.pitch; k0 += 16, ++it) {
-            const uint32_t s = it % S::CHUNKS;
-            if (it >= S::CHUNKS && !ag_wait(&cempty[s], ((it / S::CHUNKS) & 1u) ^ 1u)) { ok = false; break; }
-            const uint32_t sc = ag_smem(sS + s * S::CHUNK);
-            if (k0 + 4 * w < g.pitch) {
+  } else if (KIND != 16 && (warp == 2 || warp == 3)) {   // scales to shared memory
+    const int h = tid - 64;
+    uint32_t it = 0;
+    for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
+      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
+      // rows of w_g and rows of x, whichever is P
+      const int w0 = c.f * (FORM == FORM_YT ? PR_BM : BN);
+      const int p_lim = FORM == FORM_YT ? g.n - w0 : c.r1 - c.r0 - rank * PR_BM, q_lim = FORM == FORM_YT ? c.r1 - c.r0 : g.n - w0;
+      const int64_t wr = (int64_t)c.g * g.n + w0, xr = c.r0 + rank * PR_BM;
+      const uint8_t* ps = (FORM == FORM_YT ? g.sb + wr * g.pitch : g.sa + xr * g.pitch);
+      const uint8_t* qs = (FORM == FORM_YT ? g.sa + xr * g.pitch : g.sb + wr * g.pitch);
+      // 8 rows x 16 bytes a warp and step: thread h has word h % 4 of the rows h / 4, h / 4 + 16, ...
+      const int r0 = h >> 2, w = h & 3;
+      for (int k0 = 0; k0 < g.pitch; k0 += 16, ++it) {
+        const uint32_t s = it % S::CHUNKS;
+        if (it >= S::CHUNKS && !ag_wait(&cempty[s], ((it / S::CHUNKS) & 1u) ^ 1u)) { ok = false; break; }
+        const uint32_t sc = ag_smem(sS + s * S::CHUNK);
+        if (k0 + 4 * w < g.pitch) {
 #pragma unroll
-              for (int i = 0; i < (PR_BM + BN) / 16; ++i) {
-                const bool is_p = i < PR_BM / 16;
-                const int r = r0 + 16 * (is_p ? i : i - PR_BM / 16);
-                const uint32_t part = is_p ? w : 4 + w * S::QCH + (r >> 7);
-                // (the scales of rows that are not there are left as they are: they touch only what is not stored)
-                if (r < (is_p ? p_lim : q_lim))
-                  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 512 * part + (r & 31) * 16 + ((r >> 5) & 3) * 4),
-                               "l"((is_p ? ps : qs) + (int64_t)r * g.pitch + k0 + 4 * w)
-                               : "memory");
-              }
-            }
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ag_smem(&cfull[s])) : "memory");
-          }
-        } else {
-          const int len = FORM == FORM_DW ? c.r1 - c.r0 : red;
-          // every block is passed on, whole or not: a wait that skipped blocks could not tell a
-          // stage's next filling from the one after
-          for (int k0 = 0; k0 < len; k0 += BK, ++it) {
-            const int s = (int)(it % STAGES), tail = len - k0;
-            if (!__all_sync(0xffffffffu, pr_wait_long(&full[s], (it / STAGES) & 1u, failed))) { ok = false; break; }
-            if (FORM == FORM_DW && tail < BK) {
-              // steps tail .. of every block of 64 values, up to the last that an MMA reads: 128 bytes each, the
-              // swizzle stays within them
-              const int v = (h & 7) * 16, last = (tail + SUB - 1) / SUB * SUB;
-              for (int k = tail + (h >> 3); k < last; k += PR_HELPERS / 8) {
-#pragma unroll
-                for (int b = 0; b < PR_BM / 64; ++b) *(uint4*)(sP + s * S::P_BYTES + b * 8192 + k * 128 + v) = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int b = 0; b < S::QR / 64; ++b) *(uint4*)(sQ + s * S::Q_BYTES + b * 8192 + k * 128 + v) = make_uint4(0, 0, 0, 0);
-              }
-              if (PAIR) pr_release_cluster();
-              pr_proxy_fence();
-            }
-            __syncwarp();
-            if (lane == 0) {
-              if (PAIR) pr_arrive_leader(&fixed[s]);
-              else pr_arrive(&fixed[s]);
-            }
+          for (int i = 0; i < (PR_BM + BN) / 16; ++i) {
+            const bool is_p = i < PR_BM / 16;
+            const int r = r0 + 16 * (is_p ? i : i - PR_BM / 16);
+            const uint32_t part = is_p ? w : 4 + w * S::QCH + (r >> 7);
+            // (the scales of rows that are not there are left as they are: they touch only what is not stored)
+            if (r < (is_p ? p_lim : q_lim))
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 512 * part + (r & 31) * 16 + ((r >> 5) & 3) * 4),
+                           "l"((is_p ? ps : qs) + (int64_t)r * g.pitch + k0 + 4 * w)
+                           : "memory");
           }
         }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ag_smem(&cfull[s])) : "memory");
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      if (!ok) *failed = 1;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok) *failed = 1;
+  } else if (RELAY && warp >= RELAY_WARP && warp < RELAY_WARP + RELAYS) {   // landed stages, passed on
+    const int h = tid - RELAY_WARP * 32;
+    uint32_t it = 0;
+    for (int r = 0, t; (t = T.template at<FORM>(r)) < T.total && ok; ++r) {
+      const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
+      const int len = FORM == FORM_DW ? c.r1 - c.r0 : red;
+      // every block is passed on, whole or not: a wait that skipped blocks could not tell a
+      // stage's next filling from the one after
+      for (int k0 = 0; k0 < len; k0 += BK, ++it) {
+        const int s = (int)(it % STAGES), tail = len - k0;
+        if (!__all_sync(0xffffffffu, pr_wait_long(&full[s], (it / STAGES) & 1u, failed))) { ok = false; break; }
+        if (FORM == FORM_DW && tail < BK) {
+          // steps tail .. of every block of 64 values, up to the last that an MMA reads: 128 bytes each, the
+          // swizzle stays within them
+          const int v = (h & 7) * 16, last = (tail + SUB - 1) / SUB * SUB;
+          for (int k = tail + (h >> 3); k < last; k += PR_HELPERS / 8) {
+#pragma unroll
+            for (int b = 0; b < PR_BM / 64; ++b) *(uint4*)(sP + s * S::P_BYTES + b * 8192 + k * 128 + v) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int b = 0; b < S::QR / 64; ++b) *(uint4*)(sQ + s * S::Q_BYTES + b * 8192 + k * 128 + v) = make_uint4(0, 0, 0, 0);
+          }
+          if (PAIR) pr_release_cluster();
+          pr_proxy_fence();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) pr_arrive_leader(&fixed[s]);
+          else pr_arrive(&fixed[s]);
+        }
+      }
+    }
+    if (!ok) *failed = 1;
   } else if (warp >= 4 && warp < 12) {   // results
     const int ew = warp - 4, quarter = ew & 3, half = ew >> 2;
     unsigned char* stg = staging + ew * 2048;

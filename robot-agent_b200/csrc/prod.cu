@@ -107,7 +107,7 @@ static int launch(const char* who, const Operands& o, ProdArgs g, int type, cuda
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(PAIR ? 2 * std::min<int64_t>(sms / 2, row_tiles * per) : std::min<int64_t>(sms, row_tiles * per)));
-  cfg.blockDim = dim3(PR_THREADS(KIND));
+  cfg.blockDim = dim3(PR_THREADS(KIND, PAIR));
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -146,7 +146,7 @@ struct TileCost {
   }
   double narrow(int64_t wide, int bn) const { return of(bn, (wide + PR_BM - 1) / PR_BM, sms, PR_BM + bn); }    // FORM_YT
   double single(int64_t wide, int bn) const { return of(PR_BM, (wide + bn - 1) / bn, sms, PR_BM + bn); }
-  double pair(int64_t wide) const { return of(2 * PR_BM, (wide + 255) / 256, sms / 2, 256); }
+  double pair(int64_t wide, int bn) const { return of(2 * PR_BM, (wide + bn - 1) / bn, sms / 2, PR_BM + bn / 2); }
 };
 
 extern "C" {
@@ -174,7 +174,7 @@ int smg_group_product(const void* x, int64_t ldx, const void* w, int64_t ldw, in
   }
   int dev;
   const TileCost c = {rows, n_groups, std::max(sm_count(&dev), 2)};
-  const double t[] = {c.narrow(n, 32), c.narrow(n, 64), c.narrow(n, 128), c.single(n, 192), c.single(n, 256), c.pair(n)};
+  const double t[] = {c.narrow(n, 32), c.narrow(n, 64), c.narrow(n, 128), c.single(n, 192), c.single(n, 256), c.pair(n, 256)};
   switch (std::min_element(t, t + 6) - t) {
     case 0: return launch<16, 32, FORM_YT>(who, o, g, type, st);
     case 1: return launch<16, 64, FORM_YT>(who, o, g, type, st);
@@ -201,7 +201,7 @@ int smg_group_product_dx(const void* dy, int64_t lddy, const void* w, int64_t ld
   const cudaStream_t st = (cudaStream_t)stream;
   int dev;
   const TileCost c = {rows, n_groups, std::max(sm_count(&dev), 2)};
-  const double t[] = {c.single(k, 128), c.single(k, 192), c.single(k, 256), c.pair(k)};
+  const double t[] = {c.single(k, 128), c.single(k, 192), c.single(k, 256), c.pair(k, 256)};
   switch (std::min_element(t, t + 4) - t) {
     case 0: return launch<16, 128, FORM_DX>(who, o, g, type, st);
     case 1: return launch<16, 192, FORM_DX>(who, o, g, type, st);
@@ -260,13 +260,14 @@ int smg_mx_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_
   const cudaStream_t st = (cudaStream_t)stream;
   int dev;
   const TileCost c = {rows, n_groups, std::max(sm_count(&dev), 2)};
-  const double t[] = {c.narrow(n, 32), c.narrow(n, 64), c.narrow(n, 128), c.single(n, 192)};
-  switch (std::min_element(t, t + 4) - t) {
+  const double t[] = {c.narrow(n, 32), c.narrow(n, 64), c.narrow(n, 128), c.single(n, 192), c.pair(n, 192)};
+  switch (std::min_element(t, t + 5) - t) {
     case 0: return bits == 4 ? launch<4, 32, FORM_YT>(who, o, g, 0, st) : launch<8, 32, FORM_YT>(who, o, g, 0, st);
     case 1: return bits == 4 ? launch<4, 64, FORM_YT>(who, o, g, 0, st) : launch<8, 64, FORM_YT>(who, o, g, 0, st);
     case 2: return bits == 4 ? launch<4, 128, FORM_YT>(who, o, g, 0, st) : launch<8, 128, FORM_YT>(who, o, g, 0, st);
+    case 3: return bits == 4 ? launch<4, 192, FORM_Y>(who, o, g, 0, st) : launch<8, 192, FORM_Y>(who, o, g, 0, st);
+    default: return bits == 4 ? launch<4, 192, FORM_Y, true>(who, o, g, 0, st) : launch<8, 192, FORM_Y, true>(who, o, g, 0, st);
   }
-  return bits == 4 ? launch<4, 192, FORM_Y>(who, o, g, 0, st) : launch<8, 192, FORM_Y>(who, o, g, 0, st);
 }
 
 }   // extern "C"

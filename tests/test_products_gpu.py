@@ -309,6 +309,13 @@ def test_scores_many_tiles_of_short_rows(bits, k):
     check_scores([300, 0, 500, 201], 15001, k, bits, HF)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("counts,n,k", [([3000, 0, 2500, 700], 700, 640), ([6000], 1152, 1152), ([2049, 4000], 481, 2080)])
+def test_scores_of_many_rows(bits, counts, n, k):
+    """Tiles of two CTAs: ragged groups, a last tile of few columns, several chunks of scales."""
+    check_scores(counts, n, k, bits, BF if n == 700 else None)
+
+
 def test_scores_spread_of_magnitudes():
     """Blocks of very different sizes in one row: the scales' exponents add up right."""
     for bits in (4, 8):

@@ -621,6 +621,48 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
       const int col0 = FORM == FORM_DW ? c.f / g.p_tiles * BN : c.f * (FORM == FORM_YT ? PR_BM : BN);
       const int col_lim = FORM == FORM_Y || FORM == FORM_YT ? g.n : g.k;
       const int64_t y0 = FORM == FORM_DW ? (int64_t)c.g * g.y_stride : 0;
+      if (FORM != FORM_YT && BN >= 64 && g.y_type != SMG_EMB_F32 && g.y_vec && col0 + BN <= col_lim && !none) {
+        // 16-bit results of a tile that is whole in its columns: the places of the lane's 4 rows are found once
+        const int q = lane & 3, r0 = lane >> 2;
+        uint16_t* o = (uint16_t*)g.y + y0 + (int64_t)(row0 + quarter * 32 + r0) * g.ldy + col0 + half * (BN / 2) + q * 8;
+        const int64_t step = 8 * g.ldy;
+        const int left = row_lim - row0 - quarter * 32 - r0;   // rows r0 + 8 i below it are there
+        unsigned char* in = stg + r0 * 64 + ((q ^ (r0 >> 1)) & 3) * 16;
+        const bool bf = g.y_type == SMG_EMB_BF16;
+#pragma unroll 1
+        for (int c = 0; c < BN / 2; c += 32) {
+          uint32_t v[32], w[16];
+          ag_tmem_ld32(d + half * (BN / 2) + c, v);
+          if (bf) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              w[i] = *(const uint32_t*)&b;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const __half2 b = __floats2half2_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              w[i] = *(const uint32_t*)&b;
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *(uint4*)(stg + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)   // 8 rows on, the swap of parts is the same: (r + 8) / 2 = r / 2 + 4
+            if (8 * i < left) *(uint4*)(o + i * step + c) = *(const uint4*)(in + i * 512);
+        }
+        ag_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) pr_arrive_leader(&tempty[acc]);
+          else pr_arrive(&tempty[acc]);
+        }
+        continue;
+      }
       constexpr int HALF = BN >= 64 ? BN / 2 : BN;         // columns of D that a warp takes
       if (BN >= 64 || half == 0) {
         for (int c0 = half * HALF; c0 < half * HALF + HALF; c0 += 32) {

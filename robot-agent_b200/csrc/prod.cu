@@ -132,8 +132,9 @@ static ProdArgs prod_fill(const int32_t* off, int n_groups, int rows, int n, int
 }
 
 // Which tile: the one with the least estimated time, (rounds of tiles over the SMs) x (rows of operands
-// that a CTA loads for a tile), since every form is held up by its loads (the 128 x 256 tile of one CTA
-// takes its 384 rows at 55 bytes a cycle and SM, the pair's 256 rows at 45; the MMAs would take 100).  The groups'
+// that a CTA loads for a tile) / (bytes a cycle that it gets), since every form is held up by its loads and their
+// way through shared memory: the 128 x 256 tile of one CTA takes its 384 rows at 55 bytes a cycle
+// and SM, the pair's 256 rows at 45; the MMAs would take 100.  The groups'
 // sizes are known on the device only: they are taken to be spread about their mean, half a tile of each
 // group left over.
 struct TileCost {
@@ -146,7 +147,7 @@ struct TileCost {
   }
   double narrow(int64_t wide, int bn) const { return of(bn, (wide + PR_BM - 1) / PR_BM, sms, PR_BM + bn); }    // FORM_YT
   double single(int64_t wide, int bn) const { return of(PR_BM, (wide + bn - 1) / bn, sms, PR_BM + bn); }
-  double pair(int64_t wide, int bn) const { return of(2 * PR_BM, (wide + bn - 1) / bn, sms / 2, PR_BM + bn / 2); }
+  double pair(int64_t wide, int bn) const { return of(2 * PR_BM, (wide + bn - 1) / bn, sms / 2, PR_BM + bn / 2) * 55 / 45; }
 };
 
 extern "C" {
@@ -234,7 +235,7 @@ int smg_group_product_dw(const void* dy, int64_t lddy, const void* x, int64_t ld
   const auto cost = [&](int rt, int bn, int units, int loaded) {
     return std::ceil((double)n_groups * ((n + rt - 1) / rt) * ((k + bn - 1) / bn) / units) * loaded;
   };
-  const double t[] = {cost(128, 128, sms, 256), cost(128, 256, sms, 384), cost(256, 256, sms / 2, 256)};
+  const double t[] = {cost(128, 128, sms, 256), cost(128, 256, sms, 384), cost(256, 256, sms / 2, 256) * 55 / 45};
   switch (std::min_element(t, t + 3) - t) {
     case 0: return launch<16, 128, FORM_DW>(who, o, g, type, st);
     case 1: return launch<16, 256, FORM_DW>(who, o, g, type, st);

@@ -323,7 +323,9 @@ DEV void mx_place(int64_t t, int64_t n, const MxDiv& d, int64_t& row, int& j) {
 }
 
 // MX_EACH parts of 8 values a thread, a block's width apart; all loads first.  Bound by memory: per value
-// it reads the input once and writes bits / 8 + 1/32 bytes (and 2 with `values`).
+// it reads the input once and writes bits / 8 + 1/32 bytes (and 2 with `values`).  Measured on 16384 x 1152 bf16 in 4 bits
+// with values: 16 us, 5.3 TB/s (81% of a copy's; the rest is the launch: 65536 rows run at 5.4); a form with one
+// part a thread, a 64-bit division and codes decoded one by one had 235 instructions a part and took 20.
 #define MX_EACH 4
 template <int TYPE, int BITS, bool VEC>
 __global__ void __launch_bounds__(256) k_mx_quantise(const typename Elem<TYPE>::T* x, int64_t ldx, int rows, int64_t n, MxDiv div, MxOut o) {

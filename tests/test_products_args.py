@@ -1,11 +1,22 @@
 """Refusals of the embedding heads' C entry points, which need no GPU: bad sizes, types, alignment and null
 pointers come back as error codes with a text, before anything is launched."""
 import ctypes as C
+import os
 
 import pytest
 
+from conftest import ROOT
+
 F32, BF16 = 0, 1
 ARGS, CAPACITY = -1, -3
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _built():
+    pkg = os.path.join(ROOT, "robot-agent_b200")
+    for f in ("libsmg.so", os.path.join("scenemap_b200", "_heads.so")):
+        if not os.path.exists(os.path.join(pkg, f)):
+            pytest.skip(f"{f} not built (python __graft_entry__.py build)")
 
 
 @pytest.fixture(scope="module")

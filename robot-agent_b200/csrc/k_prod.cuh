@@ -26,7 +26,7 @@
 //               (cfull / cempty), 16 bytes of a row at a time, put into the order that the tensor memory
 //               wants (row r of 128 at 16 (r % 32) + 4 (r / 32) of 512 bytes for each 4 blocks).  DW: zeros over the
 //               rows past the group's end in its last block, where the load brought the next group's
-//               rows (in both operands, since zero times NaN is NaN), reported on fixed[s];
+//               rows (in both operands, since zero times NaN is NaN), reported on fixed[s].
 //               Pairs: warp 2 (microscaled rows: warp 13) passes a landed stage on to the leader's fixed[s];
 //   warp 12     (microscaled rows) copies landed scales to tensor memory, two chunks in turn (cready / cdone): in
 //               the MMA warp the copies and their waits took 300 cycles of the 384 that a stage has;
@@ -36,8 +36,7 @@
 // of P and one half of Q and keeps the sums of its rows; rank 0 issues the MMAs of both, which read
 // each half of Q once for the two.  That is what the single form lacks: at 128 x 256 a CTA writes 48 KB into
 // shared memory and reads 48 KB out of it for 512 cycles of MMAs, 192 bytes a cycle where an SM has 128;
-// in a pair it is 32 + 32 KB (microscaled rows,
-// 128 x 192: 40 + 40 KB for 384 cycles, in a pair 28 + 28).
+// in a pair it is 32 + 32 KB (microscaled rows, 128 x 192: 40 + 40 KB for 384 cycles, in a pair 28 + 28).
 //
 // Measured (device time in a graph; 65536 x 1152 rows in 32 groups, n = k = 1152, bf16): y 133 us, dx 131, dw 140, 1.24 to 1.33
 // PFLOP/s, the tensor pipe at 82% of the launch (a plain library product of the same rows and one matrix: 159 us); e2m1
@@ -330,8 +329,6 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
     for (int a = 0; a < 2; ++a) {
       ag_mbar_init(&cdone[a], 1);
       ag_mbar_init(&cready[a], 1);
-    }
-    for (int a = 0; a < 2; ++a) {
       ag_mbar_init(&tfull[a], 1);
       ag_mbar_init(&tempty[a], PR_EPI_WARPS * (PAIR ? 2 : 1));
     }
@@ -380,16 +377,16 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
   const int rank = PAIR ? (int)pr_rank() : 0;   // which of a pair's 128 rows of P (and halves of Q) are this CTA's
   if (FORM == FORM_DW) {   // groups by length (beyond 256 of them, where no single one holds the end up, as they come)
     for (int i = tid; i < g.n_groups; i += PR_THREADS(KIND, PAIR)) {
-      int rank = i;
+      int place = i;
       if (g.n_groups <= 256) {
         const int len = s_end[i] - s_beg[i];
-        rank = 0;
+        place = 0;
         for (int o = 0; o < g.n_groups; ++o) {
           const int other = s_end[o] - s_beg[o];
-          rank += other > len || (other == len && o < i);
+          place += other > len || (other == len && o < i);
         }
       }
-      s_cum[rank] = i;
+      s_cum[place] = i;
     }
   } else if (warp == 0) {   // first row tile of every group
     int at = 0;

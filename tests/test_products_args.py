@@ -44,6 +44,7 @@ def test_group_product_refusals(L):
         assert call(**kw) == ARGS, kw
         assert text in _text(L), (kw, _text(L))
     assert call(groups=1025) == CAPACITY and "1024" in _text(L)
+    assert call(rows=0x7fffffff) == CAPACITY and "rows" in _text(L)
     assert call(rows=0, x=None, y=None) == 0          # nothing to do
 
 

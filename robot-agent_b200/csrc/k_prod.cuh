@@ -742,6 +742,31 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
                 *(uint4*)(stg + lane * 64 + ((q ^ (lane >> 1)) & 3) * 16) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
               __syncwarp();
               const int size = g.y_type == SMG_EMB_F32 ? 4 : 2, each = 16 / size;
+              if (!g.y_vec) {
+                // rows of y off 16 bytes: 32 (16 bits) or 2 x 16 neighbouring values a step, so that a store still fills
+                // whole sectors (value by value in the 16-byte order below it touched five times as many)
+                const int left = row_lim - row0 - quarter * 32, top = col0 + c0 + h0;   // rows and columns from here
+                const int64_t at = y0 + (int64_t)(row0 + quarter * 32) * g.ldy + top;
+                if (size == 2) {
+                  uint16_t* o = (uint16_t*)g.y + at + lane;
+                  const unsigned char* in = stg + (lane & 7) * 2;
+                  if (top + lane < col_lim) {
+#pragma unroll
+                    for (int r = 0; r < 32; ++r, o += g.ldy)
+                      if (r < left) *o = *(const uint16_t*)(in + r * 64 + (((lane >> 3) ^ (r >> 1)) & 3) * 16);
+                  }
+                } else {
+                  const int e = lane & 15, r0 = lane >> 4;
+                  uint32_t* o = (uint32_t*)g.y + at + r0 * g.ldy + e;
+                  const unsigned char* in = stg + r0 * 64 + (e & 3) * 4;
+                  if (top + e < col_lim) {
+#pragma unroll
+                    for (int r = 0; r < 32; r += 2, o += 2 * g.ldy)
+                      if (r + r0 < left) *o = *(const uint32_t*)(in + r * 64 + (((e >> 2) ^ (r >> 1)) & 3) * 16);
+                  }
+                }
+                continue;
+              }
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int r = i * 8 + (lane >> 2), q = lane & 3;
@@ -749,7 +774,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
                 if (row >= row_lim || col >= col_lim) continue;
                 const uint4 u = *(const uint4*)(stg + r * 64 + ((q ^ (r >> 1)) & 3) * 16);
                 unsigned char* o = (unsigned char*)g.y + (y0 + (int64_t)row * g.ldy + col) * size;
-                if (g.y_vec && col + each <= col_lim) {
+                if (col + each <= col_lim) {
                   *(uint4*)o = u;
                 } else {
                   const uint32_t uw[4] = {u.x, u.y, u.z, u.w};

@@ -44,12 +44,15 @@
 // large tiles, shared memory's bandwidth (above); microscaled rows of few stages, the results' way out through
 // shared memory; few rows, the reading of w (64 maps of 512 x 1152: 12 us for 75 MB).
 //
-// Every wait is bounded, or goes on only until another role's bounded wait has run out; then the
-// roles run out too, SMG_PROD_TIMEOUT is set, and the CTA waits (bounded) for its own copies and
-// MMAs before it frees the tensor memory.
+// Every wait is bounded: by AG_WAIT_NS where the other side owes a stage or an accumulator, by PR_LONG_NS where it
+// may rightly take a whole tile; the latter also ends when a role has given up, in either CTA of a pair
+// (pr_fail marks both: what a follower waits for, the leader's MMAs alone commit).  Then the roles run
+// out, SMG_PROD_TIMEOUT is set, and the CTA waits (bounded) for its own copies and MMAs before it
+// frees the tensor memory.
 #pragma once
 #include "k_mx.cuh"
 #include "tc_util.cuh"
+#include "wait_rules.h"
 
 enum { FORM_Y = 0, FORM_YT = 1, FORM_DX = 2, FORM_DW = 3 };
 
@@ -73,6 +76,7 @@ struct ProdArgs {
 #define PR_EPI_WARPS 8
 #define PR_SMEM_MAX 232448
 #define PR_STAGING (PR_EPI_WARPS * 2048)
+#define PR_LONG_NS 60000000000ull   // the longest tile, dw over 2^31 rows, takes 2^25 stages of 512 to 900 cycles: up to 16 s
 #define PR_GROUP_BYTES ((3 * SMG_PROD_MAX_GROUPS + 1) * 4)
 
 // KIND 16: f16 or bf16; 8, 4: microscaled
@@ -218,12 +222,22 @@ DEV bool pr_test(uint64_t* b, uint32_t parity) {
   return ok != 0;
 }
 
-// A wait that may rightly last as long as a whole tile: it goes on while no role has failed (their
-// own waits are bounded).
+// A role gives up: every role of this CTA, and of the other one of a pair, is told.  (The other CTA is there: both
+// meet at a cluster barrier before the first and after the last role.)
+template <bool PAIR>
+DEV void pr_fail(volatile int* failed) {
+  *failed = 1;
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+        "st.relaxed.cluster.shared::cluster.u32 [a], %2;\n\t}\n" ::"r"(ag_smem((const void*)failed)),
+        "r"(pr_rank() ^ 1u), "r"(1)
+        : "memory");
+}
+
 DEV bool pr_wait_long(uint64_t* b, uint32_t parity, volatile int* failed) {
-  while (!ag_wait(b, parity))
-    if (*failed) return false;
-  return true;
+  return wait_long([&] { return ag_wait(b, parity); }, [&] { return *failed != 0; }, ag_now, PR_LONG_NS);
 }
 
 // what every role knows of the tiles
@@ -372,7 +386,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
     __syncthreads();
   }
   constexpr uint32_t tmem = 0;
-  if (tid == 0 && *tmem_slot != tmem) *failed = 1;
+  if (tid == 0 && *tmem_slot != tmem) pr_fail<PAIR>(failed);
   constexpr int RT = FORM == FORM_YT ? BN : PAIR ? 2 * PR_BM : PR_BM;
   const int rank = PAIR ? (int)pr_rank() : 0;   // which of a pair's 128 rows of P (and halves of Q) are this CTA's
   if (FORM == FORM_DW) {   // groups by length (beyond 256 of them, where no single one holds the end up, as they come)
@@ -459,7 +473,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
     }
     // the last loads must have landed before the CTA ends
     for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j) ok = wait(&full[j % STAGES], (j / STAGES) & 1u) && ok;
-    if (!ok) *failed = 1;
+    if (!ok) pr_fail<PAIR>(failed);
   } else if (warp == 1 && rank == 0) {   // MMAs
     const bool one = pr_elect();
     uint32_t it = 0, j = 0, ci = 0;
@@ -509,7 +523,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
       if (one) pr_commit<PAIR>(&tfull[acc]);   // after a failed wait too: arrives when the issued MMAs are done
     }
     if (one) pr_commit<PAIR>(done);   // every issued MMA has completed before the tensor memory is freed
-    if (!wait(done, 0) || !ok) *failed = 1;
+    if (!wait(done, 0) || !ok) pr_fail<PAIR>(failed);
   } else if (warp == 12) {   // microscaled rows: scales from shared to tensor memory
     const bool one = pr_elect();
     uint32_t ci = 0;
@@ -537,7 +551,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
       }
     }
     if (one && rank == 0) pr_commit<PAIR>(done);
-    if (!ok) *failed = 1;
+    if (!ok) pr_fail<PAIR>(failed);
   } else if (KIND != 16 && (warp == 2 || warp == 3)) {   // scales to shared memory
     const int h = tid - 64;
     uint32_t it = 0;
@@ -572,7 +586,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (!ok) *failed = 1;
+    if (!ok) pr_fail<PAIR>(failed);
   } else if (RELAY && warp >= RELAY_WARP && warp < RELAY_WARP + RELAYS) {   // landed stages, passed on
     const int h = tid - RELAY_WARP * 32;
     uint32_t it = 0;
@@ -604,7 +618,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
         }
       }
     }
-    if (!ok) *failed = 1;
+    if (!ok) pr_fail<PAIR>(failed);
   } else if (warp >= 4 && warp < 12) {   // results
     const int ew = warp - 4, quarter = ew & 3, half = ew >> 2;
     unsigned char* stg = staging + ew * 2048;
@@ -613,7 +627,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t);
       const uint32_t acc = j & 1u;
       if (!__all_sync(0xffffffffu, pr_wait_long(&tfull[acc], (j >> 1) & 1u, failed) && !*failed)) {
-        if (lane == 0) *failed = 1;
+        if (lane == 0) pr_fail<PAIR>(failed);
         break;
       }
       ag_fence_after();

@@ -1,0 +1,41 @@
+"""Rules of the embedding heads' kernels that no GPU run may break on purpose, checked without one: how a role's
+waiting ends (csrc/wait_rules.h run on the host), and that the kernels' source keeps to it."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+CSRC = os.path.join(ROOT, "robot-agent_b200", "csrc")
+
+
+def _code(name):
+    """A source file without its comments."""
+    with open(os.path.join(CSRC, name)) as f:
+        return re.sub(r"//[^\n]*|/\*.*?\*/", "", f.read(), flags=re.S)
+
+
+def test_long_wait_ends(tmp_path):
+    """A wait for a whole tile ends when the tile does, when any role of the pair has given up, or at its limit."""
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    exe = str(tmp_path / "pair_wait")
+    subprocess.run([cxx, "-O1", "-std=c++17", "-o", exe, os.path.join(HERE, "pair_wait_check.cpp")], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
+
+
+def test_failure_reaches_both_ctas_of_a_pair():
+    """Every role that gives up does so through pr_fail, which marks the other CTA too."""
+    s = _code("k_prod.cuh")
+    kernel = s[s.index("__global__"):]
+    assert not re.search(r"(\*\s*failed|sh_fail)\s*=\s*1", kernel)
+    assert kernel.count("pr_fail<PAIR>(failed)") >= 7         # loads, MMAs, scales twice, relay, results, tensor memory
+    fail = s[s.index("DEV void pr_fail"):]
+    assert "st.relaxed.cluster.shared::cluster" in fail[:fail.index("\n}")]
+    assert "while (!ag_wait" not in s                         # no wait without a limit of its own

@@ -175,15 +175,24 @@ DEV uint32_t pr_rank() {
   return r;
 }
 
-// Arrival on the leader's barrier that lies where b does here.  Without cluster-wide release and acquire:
-// what it reports is data of asynchronous copies that have landed (or a read that is over), and with
-// them on every stage the products ran at 0.4 of this speed.
+// Arrival on the leader's barrier that lies where b does here.  Where it reports data of asynchronous copies that
+// have landed, or a read that is over, it goes without cluster-wide release and acquire: with them on every
+// stage the products ran at 0.4 of this speed.  RELEASE: ordinary writes to this CTA's shared memory come before it
+// (scales, the zeros of dw's last block), and the leader waits with ag_wait<true>.
+template <bool RELEASE = false>
 DEV void pr_arrive_leader(uint64_t* b) {
-  asm volatile(
-      "{\n\t.reg .b32 a;\n\t"
-      "mapa.shared::cluster.u32 a, %0, 0;\n\t"
-      "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(ag_smem(b))
-      : "memory");
+  if constexpr (RELEASE)
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(ag_smem(b))
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+        "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(ag_smem(b))
+        : "memory");
 }
 
 // arrives on b here (PAIR: there and here) when the MMAs issued so far are done
@@ -196,9 +205,6 @@ DEV void pr_commit(uint64_t* b) {
   else
     ag_commit(b);
 }
-
-// the same after ordinary writes to shared memory that the leader's MMAs read
-DEV void pr_release_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 
 template <bool PAIR>
 DEV void pr_cluster_sync() {
@@ -438,6 +444,8 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
     return PAIR && (FORM == FORM_Y ? g.n : g.k) - (FORM == FORM_DW ? c.f / g.p_tiles : c.f) * BN <= BN / 2;
   };
   const auto wait = [](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, ag_wait(b, parity)) != 0; };
+  // for ordinary writes of either CTA of a pair
+  const auto wait_pair = [](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, ag_wait<PAIR>(b, parity)) != 0; };
   if (warp == 0) {   // loads
     const bool one = pr_elect();
     uint32_t it = 0;
@@ -491,7 +499,8 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
         const uint32_t ph = (it / STAGES) & 1u;
         const int left = len - kb * BK;
         uint64_t* landed = RELAY ? fixed : full;
-        if (!__all_sync(0xffffffffu, ready) && !wait(&landed[s], ph)) { ok = false; break; }
+        const bool zeros = PAIR && FORM == FORM_DW && left < BK;   // the other CTA has written zeros into its part
+        if (zeros ? !wait_pair(&landed[s], ph) : !__all_sync(0xffffffffu, ready) && !wait(&landed[s], ph)) { ok = false; break; }
         if (KIND != 16 && kb % S::CHUNK_STAGES == 0 && !wait(&cready[ci & 1u], (ci >> 1) & 1u)) { ok = false; break; }
         ready = pr_test(&landed[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u);   // the next stage, while this one's MMAs go out
         ag_fence_after();
@@ -535,10 +544,10 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
         if (!wait(&cfull[s], ph)) { ok = false; break; }
         pr_proxy_fence();   // they were written by ordinary copies
         if (PAIR && rank == 1) {
-          if (one) pr_arrive_leader(&cpeer[s]);
+          if (one) pr_arrive_leader<true>(&cpeer[s]);
           continue;
         }
-        if (PAIR && !wait(&cpeer[s], ph)) { ok = false; break; }
+        if (PAIR && !wait_pair(&cpeer[s], ph)) { ok = false; break; }
         ag_fence_after();
         if (one) {
           const unsigned char* sc = sS + s * S::CHUNK;
@@ -608,12 +617,12 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
 #pragma unroll
             for (int b = 0; b < S::QR / 64; ++b) *(uint4*)(sQ + s * S::Q_BYTES + b * 8192 + k * 128 + v) = make_uint4(0, 0, 0, 0);
           }
-          if (PAIR) pr_release_cluster();
           pr_proxy_fence();
         }
         __syncwarp();
         if (lane == 0) {
-          if (PAIR) pr_arrive_leader(&fixed[s]);
+          if (PAIR && FORM == FORM_DW && tail < BK) pr_arrive_leader<true>(&fixed[s]);
+          else if (PAIR) pr_arrive_leader(&fixed[s]);
           else pr_arrive(&fixed[s]);
         }
       }

@@ -26,25 +26,37 @@ DEV void ag_expect_tx(uint64_t* b, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(ag_smem(b)), "r"(bytes) : "memory");
 }
 
+// CLUSTER: acquires what another CTA of the cluster released (see pr_arrive_leader)
+template <bool CLUSTER = false>
 DEV bool ag_try_wait(uint64_t* b, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(ag_smem(b)), "r"(parity)
-      : "memory");
+  if constexpr (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(ag_smem(b)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(ag_smem(b)), "r"(parity)
+        : "memory");
   return ok != 0;
 }
 
 // bounded wait on phase `parity`; false after AG_WAIT_NS.  The clock is read only when the first try has
 // failed: reading it takes as long as several MMAs.
+template <bool CLUSTER = false>
 DEV bool ag_wait(uint64_t* b, uint32_t parity) {
-  if (ag_try_wait(b, parity)) return true;
+  if (ag_try_wait<CLUSTER>(b, parity)) return true;
   const uint64_t t0 = ag_now();
   for (uint32_t i = 0;; ++i) {
-    if (ag_try_wait(b, parity)) return true;
+    if (ag_try_wait<CLUSTER>(b, parity)) return true;
     if ((i & 255u) == 255u && ag_now() - t0 > AG_WAIT_NS) return false;
   }
 }

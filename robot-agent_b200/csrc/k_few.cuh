@@ -43,7 +43,7 @@ DEV void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t 
 template <int TYPE>
 DEV uint4 few_load(const typename Elem<TYPE>::T* row, int c, int k, bool there) {
   if (!there || c >= k) return make_uint4(0, 0, 0, 0);
-  if (c + 8 <= k) return __ldg((const uint4*)(row + c));
+  if (c + 8 <= k) return *(const uint4*)(row + c);
   Raw8<TYPE> q;
   q.template load<false>(row + c, k - c);
   return q.q[0];

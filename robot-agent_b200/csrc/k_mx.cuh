@@ -20,7 +20,9 @@
 #endif
 
 // Programmatic launch: a kernel may be set up while the one before it in the stream still runs.  It
-// touches global memory only after heads_wait(), which returns when that one is complete, its writes included.
+// touches global memory only after heads_wait(), which returns when that one is complete, its writes included, and
+// reads it with ordinary loads: the read-only path (__ldg) is for memory that nobody writes in a kernel's lifetime,
+// which begins before the wait.
 DEV void heads_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 DEV void heads_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -56,7 +58,7 @@ struct Raw8 {
   DEV void load(const T* p, int n) {   // p is used only where n > 0
     if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = n > 0 ? __ldg((const uint4*)p + i) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = n > 0 ? ((const uint4*)p)[i] : make_uint4(0, 0, 0, 0);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[i] = i < n ? p[i] : Elem<TYPE>::down(0.f);
@@ -94,7 +96,7 @@ struct Any8 {
     in = n > 0 && a >= lo && a + 16 * (V + 1) <= hi;
 #pragma unroll
     for (int i = 0; i <= V; ++i) {
-      const uint4 q = in ? __ldg((const uint4*)a + i) : make_uint4(0, 0, 0, 0);
+      const uint4 q = in ? ((const uint4*)a)[i] : make_uint4(0, 0, 0, 0);
       w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
     }
   }
@@ -373,8 +375,8 @@ __global__ void __launch_bounds__(256) k_mx_values(MxOut o, int64_t n, MxDiv div
     mx_place(t0 + i * 256, n, div, row, j);
     const uint8_t* d = o.codes + (row * o.kb * 4 + j) * BITS;
     uint32_t c[2], q[4];
-    c[0] = __ldg((const uint32_t*)d);
-    c[1] = BITS == 8 ? __ldg((const uint32_t*)d + 1) : 0u;
+    c[0] = ((const uint32_t*)d)[0];
+    c[1] = BITS == 8 ? ((const uint32_t*)d)[1] : 0u;
     const uint32_t s = o.scales[row * o.pitch + (j >> 2)];
     float u[8];
     if (TYPE == SMG_EMB_BF16) {

@@ -51,3 +51,11 @@ def test_ordinary_writes_cross_a_pair_with_release_and_acquire():
     relay = s[s.index("RELAY && warp"):]
     relay = relay[relay.index("make_uint4(0, 0, 0, 0)"):]
     assert re.search(r"tail < BK\)\s*pr_arrive_leader<true>\(&fixed", relay) and re.search(r"zeros \? !wait_pair\(&landed", s)
+
+
+@pytest.mark.parametrize("name", ["k_mx.cuh", "k_norm.cuh", "k_few.cuh", "k_prod.cuh"])
+def test_no_read_only_loads_under_programmatic_launch(name):
+    """A kernel that starts before the one that writes its inputs has ended must not read them by the non-coherent path, which
+    is for memory that nobody writes while the kernel runs (weights and gains too: a training step writes them)."""
+    s = _code(name)
+    assert "__ldg" not in s and "ld.global.nc" not in s and "__restrict__" not in s

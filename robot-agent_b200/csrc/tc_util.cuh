@@ -26,14 +26,14 @@ DEV void ag_expect_tx(uint64_t* b, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(ag_smem(b)), "r"(bytes) : "memory");
 }
 
-// CLUSTER: acquires what another CTA of the cluster released (see pr_arrive_leader)
+// CLUSTER: a relaxed look, strong towards an arrival from another CTA of the cluster (a fence orders what follows)
 template <bool CLUSTER = false>
 DEV bool ag_try_wait(uint64_t* b, uint32_t parity) {
   uint32_t ok;
   if constexpr (CLUSTER)
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(ok)
         : "r"(ag_smem(b)), "r"(parity)

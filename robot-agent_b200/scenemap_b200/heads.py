@@ -44,9 +44,11 @@ class MapHeads:
         e = f.values.float() * scale - target.float()
         rows = max(1, z.shape[0])
         loss = 0.5 * e.square().sum() / rows
-        _, dw, dgain = self.backward((e * (scale / rows)).to(z.dtype), f, z, off)
-        self.master.sub_(dw, alpha=lr)
-        self.gain.sub_(dgain, alpha=lr)
+        # The gradient for the values is e * scale / rows.  Its factor stays out of the 16-bit steps: a mean over many
+        # rows would put f16's values below its smallest ones (65536 rows x 1152: 9 of 10 were lost).
+        _, dw, dgain = self.backward(e.to(z.dtype), f, z, off)
+        self.master.sub_(dw, alpha=lr * scale / rows)
+        self.gain.sub_(dgain, alpha=lr * scale / rows)
         self.w.copy_(self.master)
         return loss
 

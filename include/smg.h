@@ -603,7 +603,8 @@ int smg_mx_product(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_
                    int32_t* err, void* stream);
 
 /* h = x + r (r may be NULL: h = x); y = h * rstd * gain with rstd = 1 / sqrt(mean(h^2) + eps), in 32
- * bits from the unrounded sum.  x, r, h rows x dim of `type`; gain dim floats.  Outputs, each may be
+ * bits from the unrounded sum; rows whose squares leave the 32-bit range are summed over a power of two, so only
+ * rstd itself need be a float.  x, r, h rows x dim of `type`; gain dim floats.  Outputs, each may be
  * NULL: h, rstd (rows floats), codes and scales of y as above (bits 4 or 8), values of those codes
  * (bf16, packed); not codes and values both.  dim <= 16384. */
 int smg_norm_add(const void* x, int64_t ldx, const void* r, int64_t ldr, const float* gain, int rows, int dim, int type, float eps,

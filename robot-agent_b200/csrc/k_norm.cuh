@@ -11,6 +11,8 @@
 // column sums leave registers for two blocks an SM); one row 2.0 us.  With the loads of a row in branches (rows off
 // 16 bytes value by value) the same took 177 and 731.
 #pragma once
+#include <math.h>
+
 #include "k_mx.cuh"
 
 struct NormArgs {
@@ -28,11 +30,14 @@ struct NormArgs {
 #define NORM_THREADS 256
 #define NORM_ROWS(WARPS) (8 / (WARPS))   // rows a block works on at a time
 
-// sum over the WARPS warps that share a row (their own named barrier; scr: WARPS floats of theirs)
-template <int WARPS>
+// sum (MAX: maximum) over the WARPS warps that share a row (their own named barrier; scr: WARPS floats of theirs)
+template <int WARPS, bool MAX = false>
 DEV float row_sum(float v, float* scr, int sub) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 16; o > 0; o >>= 1) {
+    const float u = __shfl_xor_sync(0xffffffffu, v, o);
+    v = MAX ? fmaxf(v, u) : v + u;
+  }
   if constexpr (WARPS > 1) {
     const int w = (threadIdx.x >> 5) % WARPS;
     asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "r"(WARPS * 32) : "memory");   // the last sum has been read
@@ -40,7 +45,7 @@ DEV float row_sum(float v, float* scr, int sub) {
     asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "r"(WARPS * 32) : "memory");
     v = 0.f;
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) v += scr[i];
+    for (int i = 0; i < WARPS; ++i) v = MAX ? fmaxf(v, scr[i]) : v + scr[i];
   }
   return v;
 }
@@ -96,7 +101,7 @@ DEV float rstd_of(float ss, float dim, float eps, float& low) {
   const float v = q + eps, b = v - q, ve = ((q - (v - b)) + (eps - b)) + qe;
   const float r = 1.f / sqrtf(v), t = v * r, te = __fmaf_rn(v, r, -t);
   const float e = __fmaf_rn(-ve * r, r, __fmaf_rn(-te, r, __fmaf_rn(-t, r, 1.f)));
-  low = 0.5f * r * e;
+  low = r > 0.f ? 0.5f * r * e : 0.f;   // an infinity in the row: 1 / rms is 0 and lacks nothing
   return r;
 }
 
@@ -128,18 +133,38 @@ __global__ void __launch_bounds__(NORM_THREADS) k_norm_add(NormArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) h[i][k] = a.r ? x[i].get(k) + r[i].get(k) : x[i].get(k);
   }
-  float sq[8];   // 8 short sums, then their tree: fewer roundings than one long sum
+  const auto squares = [&](float by) {   // sum of the row's (h * by)^2
+    float sq[8];   // 8 short sums, then their tree: fewer roundings than one long sum
 #pragma unroll
-  for (int k = 0; k < 8; ++k) sq[k] = h[0][k] * h[0][k];
+    for (int k = 0; k < 8; ++k) sq[k] = (h[0][k] * by) * (h[0][k] * by);
 #pragma unroll
-  for (int i = 1; i < NV; ++i)
+    for (int i = 1; i < NV; ++i)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sq[k] = __fmaf_rn(h[i][k], h[i][k], sq[k]);
-  const float ss = row_sum<WARPS>(((sq[0] + sq[1]) + (sq[2] + sq[3])) + ((sq[4] + sq[5]) + (sq[6] + sq[7])), scr[sub], sub);
+      for (int k = 0; k < 8; ++k) sq[k] = __fmaf_rn(h[i][k] * by, h[i][k] * by, sq[k]);
+    return row_sum<WARPS>(((sq[0] + sq[1]) + (sq[2] + sq[3])) + ((sq[4] + sq[5]) + (sq[6] + sq[7])), scr[sub], sub);
+  };
+  const float ss = squares(1.f);
   // The codes' rounding turns an error of the last place into one of a code, so 1 / rms goes in two parts: what
   // remains are the two products' own roundings (carrying those on too changed next to no code).
   float low;
-  const float rstd = rstd_of(ss, (float)a.dim, a.eps, low);
+  float rstd = rstd_of(ss, (float)a.dim, a.eps, low);
+  if constexpr (TYPE != SMG_EMB_F16) {
+    // Squares beyond 2^127, or so small that those below 2^-126 are missed (f16 has neither): once more with the row over a
+    // power of two, by its largest magnitude or the root of eps, whichever is more.  All threads of a row together.
+    if (!(rstd > 0.f && rstd < 0x1p40f)) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(h[i][k]));
+      m = fmaxf(row_sum<WARPS, true>(m, scr[sub], sub), sqrtf(a.eps));
+      if (m < INFINITY) {
+        const float by = mx_two(127 - (int)(__float_as_uint(m) >> 23));
+        rstd = rstd_of(squares(by), (float)a.dim, a.eps * by * by, low) * by;
+        low *= by;
+      }
+    }
+  }
   if (a.rstd && t == 0) a.rstd[row] = rstd;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {

@@ -38,7 +38,8 @@ class MapHeads:
 
     def train_step(self, z: torch.Tensor, target: torch.Tensor, off: torch.Tensor, lr: float) -> torch.Tensor:
         """One step of gradient descent on the mean over the rows of |y / sqrt(dim) - target|^2 / 2, target the unit vector of
-        the object that row r shows.  Returns the loss (a tensor: nothing waits for it)."""
+        the object that row r shows.  Returns the loss (a tensor: nothing waits for it).  A step that finds the device's
+        error word set (products.error: bad offsets, a wait that ran out) changes nothing and returns NaN."""
         f = self.forward(z, off, 8, True)
         scale = self.dim ** -0.5                       # |y| is sqrt(dim)
         e = f.values.float() * scale - target.float()
@@ -47,10 +48,13 @@ class MapHeads:
         # The gradient for the values is e * scale / rows.  Its factor stays out of the 16-bit steps: a mean over many
         # rows would put f16's values below its smallest ones (65536 rows x 1152: 9 of 10 were lost).
         _, dw, dgain = self.backward(e.to(z.dtype), f, z, off)
+        bad = P.failed(z.device)
+        dw.masked_fill_(bad, 0)
+        dgain.masked_fill_(bad, 0)
         self.master.sub_(dw, alpha=lr * scale / rows)
         self.gain.sub_(dgain, alpha=lr * scale / rows)
         self.w.copy_(self.master)
-        return loss
+        return loss.masked_fill_(bad[0], float("nan"))
 
     def bank(self, vectors: torch.Tensor, bits: int = 4) -> P.MxRows:
         """Memory bank of the maps' object vectors (n_maps x n x dim) in microscaled rows."""

@@ -68,6 +68,12 @@ def error(device="cuda") -> int:
     return int(_heads.error_word(_index(device)).item())
 
 
+def failed(device="cuda") -> torch.Tensor:
+    """Whether the word is set by what the current stream has queued so far: a bool of one entry on the device, without
+    waiting."""
+    return _heads.error_word(_index(device)) != 0
+
+
 def clear_error(device="cuda") -> None:
     _heads.error_word(_index(device)).zero_()
 

@@ -58,3 +58,26 @@ def test_step_matches_64_bits(t, counts, dim):
     want = 0.5 * (e * e).sum() / rows
     assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
     assert P.error() == 0
+
+
+def test_step_with_bad_offsets_changes_nothing():
+    """Offsets that break the rules leave unspecified results: none of them reaches the weights or the gain, and the loss says so."""
+    import torch
+    from scenemap_b200 import products as P
+    from scenemap_b200.heads import MapHeads
+    torch.manual_seed(2)
+    P.clear_error()
+    dim, rows = 96, 300
+    H = MapHeads(2, dim)
+    z, target = unit(torch.randn(rows, dim, device="cuda")).bfloat16(), unit(torch.randn(rows, dim, device="cuda"))
+    good = torch.tensor([0, 100, rows], dtype=torch.int32, device="cuda")
+    assert torch.isfinite(H.train_step(z, target, good, 10.0))
+    before = H.master.clone(), H.gain.clone(), H.w.clone()
+    filler = torch.full((64, rows, dim), float("nan"), device="cuda")        # what unwritten outputs may hold
+    del filler
+    for off in ([0, 400, rows], [5, 100, rows], [0, 100, 200]):
+        loss = H.train_step(z, target, torch.tensor(off, dtype=torch.int32, device="cuda"), 10.0)
+        assert torch.isnan(loss) and P.error() == P.BAD_OFFSETS
+        assert all(torch.equal(a, b) for a, b in zip((H.master, H.gain, H.w), before))
+        P.clear_error()
+    assert torch.isfinite(H.train_step(z, target, good, 10.0)) and not torch.equal(H.master, before[0])

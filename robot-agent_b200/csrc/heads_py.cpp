@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -33,10 +34,23 @@ void check(const char* who, int rc) {
   if (rc != SMG_OK) throw Refusal(std::string(who) + " rc=" + std::to_string(rc) + ": " + smg_last_error());
 }
 
-const at::Tensor& tensor(const char* who, PyObject* o, const char* name) {
+// a tensor that a call keeps for itself, or got from one before
+const at::Tensor& kept(const char* who, PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse(who, std::string(name) + " must be a tensor");
   return THPVariable_Unpack(o);
 }
+
+// an input; nothing is recorded for autograd, so one that asks for it is not taken in silence
+const at::Tensor& tensor(const char* who, PyObject* o, const char* name) {
+  const at::Tensor& t = kept(who, o, name);
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    refuse(who, std::string(name) + " requires gradients, which this call does not record: call it under torch.no_grad() or with " + name +
+                    ".detach(), and the gradients' own calls for them");
+  return t;
+}
+
+// changes in place so far (inference tensors do not count theirs)
+int64_t version(const at::Tensor& t) { return t.is_inference() ? 0 : (int64_t)t._version(); }
 
 int code_of(at::ScalarType t) {
   return t == at::kFloat ? SMG_EMB_F32 : t == at::kBFloat16 ? SMG_EMB_BF16 : t == at::kHalf ? SMG_EMB_F16 : -1;
@@ -305,7 +319,10 @@ const float* gain_of(const char* who, const at::Tensor& g, const at::Tensor& x) 
 
 bool like(const at::Tensor& a, const at::Tensor& b) { return a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes(); }
 
-// (x, residual, gain, eps, bits, values) -> (h; buffer of codes, scales, 1 / rms; values; x; residual as read)
+// changes in place of both inputs of a norm, in one number
+int64_t versions(const at::Tensor& x, const at::Tensor* r) { return version(x) << 32 | (r ? version(*r) : 0); }
+
+// (x, residual, gain, eps, bits, values) -> (h; buffer of codes, scales, 1 / rms; values; x; residual as read; their versions)
 PyObject* norm_add(PyObject* const* a) {
   const char* who = "norm_add";
   const at::Tensor &x = tensor(who, a[0], "x"), &gain = tensor(who, a[2], "gain");
@@ -334,14 +351,18 @@ PyObject* norm_add(PyObject* const* a) {
         smg_norm_add(xr.t.data_ptr(), xr.ld, res ? r.t.data_ptr() : nullptr, r.ld, g, as_int(who, rows), as_int(who, dim),
                      code_of(x.scalar_type()), (float)eps, h.data_ptr(), dim, (float*)(p + cb + sb), bits, p, p + cb,
                      want ? (uint16_t*)v.data_ptr() : nullptr, stream_of(dev)));
-  return Py_BuildValue("(NNNNN)", wrap(h), wrap(buf), want ? wrap(v) : Py_NewRef(Py_None), wrap(xr.t), res ? wrap(r.t) : Py_NewRef(Py_None));
+  return Py_BuildValue("(NNNNNL)", wrap(h), wrap(buf), want ? wrap(v) : Py_NewRef(Py_None), wrap(xr.t), res ? wrap(r.t) : Py_NewRef(Py_None),
+                       (long long)versions(xr.t, res ? &r.t : nullptr));
 }
 
-// (dy, x, residual, rstd buffer, byte offset in it, gain, dh) -> (dx, dgain)
+// (dy, x, residual, rstd buffer, byte offset in it, gain, dh, versions or -1) -> (dx, dgain)
 PyObject* norm_add_backward(PyObject* const* a) {
   const char* who = "norm_add_backward";
-  const at::Tensor &dy = tensor(who, a[0], "dy"), &x = tensor(who, a[1], "x"), &buf = tensor(who, a[3], "rstd"), &gain = tensor(who, a[5], "gain");
+  const at::Tensor &dy = tensor(who, a[0], "dy"), &x = kept(who, a[1], "x"), &buf = kept(who, a[3], "rstd"), &gain = tensor(who, a[5], "gain");
   if (!like(dy, x)) refuse(who, "dy must be like x");
+  const long long was = PyLong_AsLongLong(a[7]);
+  if (was >= 0 && was != versions(x, a[2] == Py_None ? nullptr : &kept(who, a[2], "residual")))
+    refuse(who, "x or the residual was changed in place since the norm; its gradient reads them again");
   const bool res = a[2] != Py_None, past = a[6] != Py_None;
   if (past && !like(tensor(who, a[6], "dh"), x)) refuse(who, "dh must be like x");
   const float* g = gain_of(who, gain, x);
@@ -352,7 +373,7 @@ PyObject* norm_add_backward(PyObject* const* a) {
   const Device d(dev);
   const Rows yr = plain(dy), xr = plain(x);
   Rows r = {at::Tensor(), 0}, h = {at::Tensor(), 0};
-  if (res) r = plain(tensor(who, a[2], "residual"));
+  if (res) r = plain(kept(who, a[2], "residual"));
   if (past) h = plain(THPVariable_Unpack(a[6]));
   const int64_t rows = x.size(0), dim = x.size(1);
   at::Tensor dx = make({rows, dim}, x.scalar_type(), dev), dgain = make({dim}, at::kFloat, dev);
@@ -404,7 +425,7 @@ PyObject* set_error(PyObject*, PyObject* type) {
   { #name, (PyCFunction)(void (*)(void))entry<name, n>, METH_FASTCALL, nullptr }
 
 PyMethodDef methods[] = {ENTRY(grouped, 4),    ENTRY(grouped_dx, 4), ENTRY(grouped_dw, 4), ENTRY(mx_quantise, 3), ENTRY(mx_product, 11),
-                         ENTRY(mx_values, 6),  ENTRY(norm_add, 6),   ENTRY(norm_add_backward, 7), ENTRY(error_word, 1),
+                         ENTRY(mx_values, 6),  ENTRY(norm_add, 6),   ENTRY(norm_add_backward, 8), ENTRY(error_word, 1),
                          {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_heads", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -6,7 +6,8 @@ device and return new tensors.  `off` (int32, groups + 1 entries, on the device)
 of every map among the packed rows.  Inputs may have any strides: one whose rows the kernels cannot
 read (a last stride other than 1, or for the products rows off 16-byte boundaries) is laid out anew
 within the call.  error(device) reads the word in which the kernels report bad offsets; a device's first product
-makes that word, so it comes before any stream capture.
+makes that word, so it comes before any stream capture.  Nothing is recorded for autograd: inputs that require
+gradients are refused while torch records them, and the gradients are calls of their own.
 
 The steps of a call (checks, outputs, the library's call) are C++: csrc/heads_py.cpp, built in-tree
 as scenemap_b200/_heads.so over the same libsmg.so that smg.py loads.
@@ -170,12 +171,13 @@ def mx_product(a: MxRows, b: MxRows, off: torch.Tensor | None = None, out_dtype:
 
 class NormRows:
     """What norm_add() returns: the sum h, 1 / rms of every row (rstd), the normalised rows in codes (rows, and their
-    values), and the inputs that its gradient reads again."""
+    values), and the inputs that its gradient reads again (they are the caller's own tensors where their rows could be
+    read in place: norm_add_backward refuses them once they were changed in place)."""
 
-    __slots__ = ("h", "rows", "x", "residual", "_rstd")
+    __slots__ = ("h", "rows", "x", "residual", "_rstd", "_versions")
 
-    def __init__(self, h, rows, x, residual):
-        self.h, self.rows, self.x, self.residual, self._rstd = h, rows, x, residual, None
+    def __init__(self, h, rows, x, residual, versions=-1):
+        self.h, self.rows, self.x, self.residual, self._rstd, self._versions = h, rows, x, residual, None, versions
 
     @property
     def rstd(self) -> torch.Tensor:      # behind codes and scales in their buffer
@@ -191,15 +193,15 @@ class NormRows:
 def norm_add(x: torch.Tensor, residual: torch.Tensor | None, gain: torch.Tensor, eps: float = 1e-6, bits: int = 8,
              values: bool = False) -> NormRows:
     """h = x + residual and h / rms(h) * gain in microscaled rows of `bits`."""
-    h, buf, v, x, residual = _heads.norm_add(x, residual, gain, eps, bits, values)
+    h, buf, v, x, residual, versions = _heads.norm_add(x, residual, gain, eps, bits, values)
     rows, dim = x.shape
-    return NormRows(h, MxRows._of(buf, rows, dim, bits, v), x, residual)
+    return NormRows(h, MxRows._of(buf, rows, dim, bits, v), x, residual, versions)
 
 
 def norm_add_backward(dy: torch.Tensor, f: NormRows, gain: torch.Tensor, dh: torch.Tensor | None = None):
     """(dx, dgain) of norm_add(): dx is the gradient for x and for the residual alike; dh is the gradient that reaches
     h past the norm.  The rounding to codes counts as the identity."""
-    return _heads.norm_add_backward(dy, f.x, f.residual, f.rows._buf, f.rows._bytes()[1], gain, dh)
+    return _heads.norm_add_backward(dy, f.x, f.residual, f.rows._buf, f.rows._bytes()[1], gain, dh, f._versions)
 
 
 _load()

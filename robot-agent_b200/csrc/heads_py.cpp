@@ -11,6 +11,8 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/InferenceMode.h>
+#include <cuda_runtime.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -94,15 +96,32 @@ at::Tensor make(at::IntArrayRef shape, at::ScalarType t, int dev) {
 
 cudaStream_t stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
 
-// error word of each device
+// A device word of 0, made outside of what the thread may be capturing: its own allocation and stream, waited for.
+int32_t* new_word() {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  void* p = nullptr;
+  cudaStream_t s = nullptr;
+  cudaError_t e = cudaMalloc(&p, 256);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 256, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (s) cudaStreamDestroy(s);
+  if (e != cudaSuccess && p) cudaFree(p);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) throw Refusal(std::string("no error word: ") + cudaGetErrorString(e));
+  return (int32_t*)p;
+}
+
+// error word of each device (the caller has made the device current), an ordinary tensor whatever the mode
 at::Tensor& word(int dev) {
   static at::Tensor words[64];
   static std::mutex m;
-  if (dev >= 64) throw Refusal("device index above 63");
+  if (dev < 0 || dev >= 64) throw Refusal("device index outside 0 .. 63");
   std::lock_guard<std::mutex> lock(m);
   if (!words[dev].defined()) {
-    words[dev] = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, dev));
-    c10::cuda::stream_synchronize(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev));   // zero before any stream's kernel sets it
+    const c10::InferenceMode ordinary(false);
+    words[dev] = at::from_blob(new_word(), {1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)dev));
   }
   return words[dev];
 }
@@ -388,6 +407,7 @@ PyObject* norm_add_backward(PyObject* const* a) {
 
 PyObject* error_word(PyObject* const* a) {
   const int dev = (int)PyLong_AsLong(a[0]);
+  const Device d(dev);
   return wrap(word(dev));
 }
 

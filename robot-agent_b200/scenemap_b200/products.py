@@ -5,9 +5,9 @@ All tensors are torch tensors on one CUDA device; the calls run on torch's curre
 device and return new tensors.  `off` (int32, groups + 1 entries, on the device) holds the first row
 of every map among the packed rows.  Inputs may have any strides: one whose rows the kernels cannot
 read (a last stride other than 1, or for the products rows off 16-byte boundaries) is laid out anew
-within the call.  error(device) reads the word in which the kernels report bad offsets; a device's first product
-makes that word, so it comes before any stream capture.  Nothing is recorded for autograd: inputs that require
-gradients are refused while torch records them, and the gradients are calls of their own.
+within the call.  error(device) reads the word in which the kernels report bad offsets.  Nothing is
+recorded for autograd: inputs that require gradients are refused while torch records them, and the
+gradients are calls of their own.
 
 The steps of a call (checks, outputs, the library's call) are C++: csrc/heads_py.cpp, built in-tree
 as scenemap_b200/_heads.so over the same libsmg.so that smg.py loads.

@@ -588,9 +588,9 @@ int smg_group_product_dw(const void* dy, int64_t lddy, const void* x, int64_t ld
  * is above.  A block that holds an infinity or NaN gets the scale NaN.
  * codes: rows of ceil(k/32)*32*bits/8 bytes (4 bits: element 2i in the low half of byte i), zeros
  * past k.  scales: rows of ceil(k/128)*4 bytes, e + 127 (255 = NaN), zeros past the last block.
- * Both 16-byte aligned.  values (may be NULL): the values that the codes stand for, bf16 (exact but
- * for magnitudes below 2^-126), rows x k packed.  codes and scales may be NULL together when
- * values is given. */
+ * Codes start on 16 bytes and scales on 4, so any run of rows is a matrix of its own.  values (may be
+ * NULL): the values that the codes stand for, bf16 (exact but for magnitudes below 2^-126), rows x k
+ * packed.  codes and scales may be NULL together when values is given. */
 int smg_mx_quantise(const void* x, int64_t ldx, int rows, int k, int type, int bits, uint8_t* codes, uint8_t* scales,
                     uint16_t* values, void* stream);
 /* The values that microscaled rows stand for, as out_type (leading dimension ld). */

@@ -41,7 +41,8 @@ static inline int mx_args(const char* who, int rows, int k, int bits, const uint
   if (rows < 0 || k < 1 || k > (1 << 24)) return fail(SMG_ERR_ARGS, "%s: bad sizes (rows %d, %d values a row)", who, rows, k);
   if (bits != 4 && bits != 8) return fail(SMG_ERR_ARGS, "%s: bits must be 4 or 8", who);
   if (rows > 0 && (!codes != !scales)) return fail(SMG_ERR_ARGS, "%s: codes and scales go together", who);
-  if (!on16(codes) || !on16(scales)) return fail(SMG_ERR_ARGS, "%s: codes and scales must start on 16 bytes", who);
+  // the products' tensor maps want the codes on 16 bytes (rows of them are multiples of it); scales are copied 4 at a time
+  if (!on16(codes) || ((uintptr_t)scales & 3)) return fail(SMG_ERR_ARGS, "%s: codes must start on 16 bytes, scales on 4", who);
   return SMG_OK;
 }
 

@@ -98,7 +98,9 @@ def grouped_dw(dy: torch.Tensor, x: torch.Tensor, off: torch.Tensor | None, out_
 class MxRows:
     """Microscaled rows: codes (..., ceil(k/32)*32*bits/8 bytes) and scales (..., ceil(k/128)*4 bytes), both uint8;
     `values`, where asked for, is what the codes stand for (bf16).  Rows that the library makes lie in
-    one buffer, out of which the two tensors are cut when first asked for."""
+    one buffer, out of which the two tensors are cut when first asked for; a run of them, codes[i:j] and scales[i:j], is a
+    bank of its own.  Codes and scales made elsewhere must hold zeros past k and past the last block: a product
+    reads them (zero times a scale of 255, NaN, is NaN)."""
 
     __slots__ = ("_codes", "_scales", "_buf", "_shape", "bits", "k", "values")
 

@@ -17,7 +17,9 @@ extern "C" PFN_cuTensorMapEncodeTiled_v12000 smg_tmap_encoder();   // smg.cu
 static int prod_args(const char* who, const int32_t* off, int n_groups, int rows, int n, int k, int type, int out_type) {
   if (n_groups < 1 || rows < 0 || n < 1 || k < 1 || (!off && n_groups != 1))
     return fail(SMG_ERR_ARGS, "%s: bad sizes (n_groups %d, rows %d, n %d, k %d%s)", who, n_groups, rows, n, k, off ? "" : ", no offsets");
-  if (rows > 0x7ffffe00) return fail(SMG_ERR_CAPACITY, "%s: too many rows for one call", who);   // row tiles are counted in 32 bits
+  // tiles and stages are counted in 32 bits, the last one whole
+  if (rows > 0x7ffffe00) return fail(SMG_ERR_CAPACITY, "%s: too many rows for one call", who);
+  if (n > 0x7ffffe00 || k > 0x7ffffe00) return fail(SMG_ERR_CAPACITY, "%s: too wide for one call (n %d, k %d)", who, n, k);
   if (n_groups > SMG_PROD_MAX_GROUPS) return fail(SMG_ERR_CAPACITY, "%s: %d groups, at most %d", who, n_groups, SMG_PROD_MAX_GROUPS);
   if (type != SMG_EMB_BF16 && type != SMG_EMB_F16) return fail(SMG_ERR_ARGS, "%s: inputs must be bf16 or f16", who);
   if (!type_ok(out_type)) return fail(SMG_ERR_ARGS, "%s: bad output type", who);

@@ -1,5 +1,7 @@
 // C ABI of the embedding heads' row operators (include/smg.h): microscaled rows, the residual norm
 // and its gradients.
+#include <algorithm>
+
 #include "heads_host.h"
 #include "k_norm.cuh"
 
@@ -123,7 +125,7 @@ int smg_norm_add(const void* x, int64_t ldx, const void* r, int64_t ldr, const f
 #define LAUNCH(T, W, NV)                                                                                      \
   const auto f = bits == 4 ? (vec ? k_norm_add<T, 4, W, NV, true> : k_norm_add<T, 4, W, NV, false>)           \
                            : (vec ? k_norm_add<T, 8, W, NV, true> : k_norm_add<T, 8, W, NV, false>);          \
-  return launch_next(who, f, (unsigned)((rows + NORM_ROWS(W) - 1) / NORM_ROWS(W)), NORM_THREADS, 0, (cudaStream_t)stream, a)
+  return launch_next(who, f, (unsigned)(((int64_t)rows + NORM_ROWS(W) - 1) / NORM_ROWS(W)), NORM_THREADS, 0, (cudaStream_t)stream, a)
 #define CALL32(W, NV) LAUNCH(SMG_EMB_F32, W, NV)
 #define CALLBF(W, NV) LAUNCH(SMG_EMB_BF16, W, NV)
 #define CALLHF(W, NV) LAUNCH(SMG_EMB_F16, W, NV)
@@ -161,8 +163,7 @@ int smg_norm_add_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
   int parts = 0, e = SMG_OK;
   if (rows > 0) {
 #define LAUNCH(T, W, NV)                                                                         \
-  parts = (rows + NORM_ROWS(W) - 1) / NORM_ROWS(W);                                              \
-  if (parts > NORM_PARTS) parts = NORM_PARTS;                                                    \
+  parts = (int)std::min<int64_t>(((int64_t)rows + NORM_ROWS(W) - 1) / NORM_ROWS(W), NORM_PARTS); \
   const int sm = W < 8 ? NORM_ROWS(W) * dim * 4 : 0;                                             \
   e = launch_next(who, vec ? k_norm_add_bwd<T, W, NV, true> : k_norm_add_bwd<T, W, NV, false>, parts, NORM_THREADS, sm, st, a)
     if (type == SMG_EMB_F32) BY_STEPS2(steps, CALL32);

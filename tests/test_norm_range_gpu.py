@@ -68,3 +68,25 @@ def test_row_with_an_infinity(t, rows, dim):
     assert torch.equal(f.rows.codes[keep], want.rows.codes[keep]) and torch.equal(f.rows.scales[keep], want.rows.scales[keep])
     assert f.rstd[1] == 0 and f.rows.scales[1, 1] == 255 and f.values[1, 32:64].isnan().all()
     assert not f.values[1, :32].any() and not f.values[1, 64:].any()
+
+
+def test_as_many_rows_as_a_call_counts():
+    """2^31 - 1 rows of one value: the last ones are those of a small call, and the gradient's sum counts them all."""
+    rows, gain = 0x7fffffff, torch.full((1,), 1.5, device="cuda")
+    L = P._lib()
+    x = torch.zeros(rows, 1, dtype=BF, device="cuda")
+    x[-100:] = rnd(100, 1)
+    v, rstd = torch.empty_like(x), torch.empty(rows, device="cuda")
+    word = torch.cuda.current_stream().cuda_stream
+    assert L.smg_norm_add(x.data_ptr(), 1, None, 0, gain.data_ptr(), rows, 1, 1, 1e-6, None, 1, rstd.data_ptr(), 8, None, None,
+                          v.data_ptr(), word) == 0, L.smg_last_error()
+    f = P.norm_add(x[-100:], None, gain, values=True)
+    assert torch.equal(v[-100:], f.values) and torch.equal(rstd[-100:], f.rstd) and not v[:1000].any()
+    dx, dgain = v, torch.empty(1, device="cuda")           # dx over the values
+    work = torch.empty(L.smg_norm_add_bwd_work(1), dtype=torch.uint8, device="cuda")
+    assert L.smg_norm_add_bwd(x.data_ptr(), 1, x.data_ptr(), 1, None, 0, rstd.data_ptr(), gain.data_ptr(), None, 0, rows, 1, 1,
+                              dx.data_ptr(), 1, dgain.data_ptr(), work.data_ptr(), word) == 0, L.smg_last_error()
+    want = P.norm_add_backward(x[-100:], f, gain)
+    assert torch.equal(dx[-100:], want[0])
+    # zeros elsewhere: the 100 terms' sum in another order
+    assert abs(float(dgain - want[1])) <= 100 * 2.0 ** -23 * float((x[-100:].float().abs()).sum())

@@ -175,6 +175,7 @@ int as_int(const char* who, int64_t v) {
 }
 
 const int32_t* offsets(const char* who, PyObject* o, int64_t groups, int dev) {
+  if (groups < 1) refuse(who, "no groups");
   if (o == Py_None) {
     if (groups != 1) refuse(who, "several groups need offsets");
     return nullptr;

@@ -28,3 +28,15 @@ def test_scores_of_sliced_banks(bits, rows, n, k):
         R.near(y, want, mags, k, "scores")
         assert torch.equal(bank.dequantise(FP).double(), w[b0:b0 + n])
     assert P.error() == 0
+
+
+def test_offsets_without_a_group():
+    """No group at all is a refusal of the call's own, whichever tensor says so."""
+    from scenemap_b200.smg import SmgError
+    if not has_gpu():
+        pytest.skip("no GPU")
+    x, none = rnd(8, 64), torch.empty(0, dtype=torch.int32, device="cuda")
+    for call in (lambda: P.grouped_dw(x, x, none), lambda: P.grouped_dw(x, x, none[:0].new_zeros(1)),
+                 lambda: P.grouped(x, rnd(0, 16, 64), none.new_zeros(1)), lambda: P.grouped_dx(x, rnd(0, 64, 16), none.new_zeros(1))):
+        with pytest.raises(SmgError, match="group"):
+            call()

@@ -268,13 +268,22 @@ int bits_of(const char* who, PyObject* o) {
   return (int)b;
 }
 
+bool flag(const char* who, PyObject* o, const char* name) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    PyErr_Clear();
+    refuse(who, std::string(name) + " must be true or false");
+  }
+  return v == 1;
+}
+
 // (x, bits, values) -> (buffer of codes, then scales; values or None)
 PyObject* mx_quantise(PyObject* const* a) {
   const char* who = "mx_quantise";
   const at::Tensor& x = tensor(who, a[0], "x");
   if (x.dim() != 2 || code_of(x.scalar_type()) < 0 || x.size(1) < 1) refuse(who, "x must be rows x k of f32, bf16 or f16");
   const int bits = bits_of(who, a[1]), dev = on_device(who, x);
-  const bool want = PyObject_IsTrue(a[2]) == 1;
+  const bool want = flag(who, a[2], "values");
   const Device d(dev);
   const int64_t rows = x.size(0), k = x.size(1), cb = rows * code_bytes(k, bits);
   const Rows xr = plain(x);
@@ -353,7 +362,7 @@ PyObject* norm_add(PyObject* const* a) {
   same_device(who, dev, gain);
   const double eps = PyFloat_AsDouble(a[3]);
   if (eps == -1.0 && PyErr_Occurred()) { PyErr_Clear(); refuse(who, "eps must be a number"); }
-  const bool want = PyObject_IsTrue(a[5]) == 1, res = a[1] != Py_None;
+  const bool want = flag(who, a[5], "values"), res = a[1] != Py_None;
   Rows r = {at::Tensor(), 0};
   if (res) {
     const at::Tensor& t = tensor(who, a[1], "residual");

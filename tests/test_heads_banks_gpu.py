@@ -40,3 +40,14 @@ def test_offsets_without_a_group():
                  lambda: P.grouped(x, rnd(0, 16, 64), none.new_zeros(1)), lambda: P.grouped_dx(x, rnd(0, 64, 16), none.new_zeros(1))):
         with pytest.raises(SmgError, match="group"):
             call()
+
+
+def test_flags_without_a_truth_value():
+    """A flag that has no truth value is refused, not left as an exception behind a result."""
+    from scenemap_b200.smg import SmgError
+    if not has_gpu():
+        pytest.skip("no GPU")
+    x, gain, flag = rnd(8, 64), torch.ones(64, device="cuda"), torch.ones(2)
+    for call in (lambda: P.mx_quantise(x, 4, values=flag), lambda: P.norm_add(x, None, gain, values=flag)):
+        with pytest.raises(SmgError, match="values"):
+            call()

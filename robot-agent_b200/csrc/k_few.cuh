@@ -6,8 +6,9 @@
 // warps share the k axis, 32 values a step.  The order of k within an mma is free as long as both operands
 // have the same: lane l holds 8 consecutive values (one 16-byte load) of rows l / 4 and l / 4 + 8 of w, and of row l / 4 of
 // x, at 8 (l % 4), and they serve as the fragments of two m16n8k16 products.  The warps' sums are added in warp order.
-// Larger groups than 8 rows go round again (w_g's rows then come from the cache).  Measured: one row, k = 768, n = 256: 2.1 us
-// (the tcgen05 form 7.3); 24 groups of 512 x 1152: 7.2 us, 3.9 TB/s.
+// Larger groups than 8 rows go round again (w_g's rows then come from the cache), one round after the other: 512 rows all
+// in one of 64 groups of 512 x 768 take 66 us, 8 in each 14.  Measured: one row, k = 768, n = 256: 2.1 us (the tcgen05
+// form 7.3); 24 groups of 512 x 1152 (28 MB): 9.1 us from memory, 6.3 where L2 holds them.
 #pragma once
 #include "k_mx.cuh"
 

@@ -7,9 +7,10 @@
 // A row is held in registers (8 values a lane and step, h in 32 bits) between the sum of squares
 // and the outputs, so every input is read once and every output written once; both kernels are bound by
 // memory.  WARPS warps share a row: one for short rows, so that no row waits on a block barrier.  Measured on
-// 65536 x 1152 bf16: forward with codes and values 104 us (6.5 TB/s, a copy's rate), gradient 146 us (5.2 TB/s: its
+// 65536 x 1152 bf16: forward with codes and values 108 us on the device (6.3 TB/s, 96% of a copy's rate), gradient 140 us (5.4 TB/s: its
 // column sums leave registers for two blocks an SM); one row 2.0 us.  With the loads of a row in branches (rows off
-// 16 bytes value by value) the same took 177 and 731.
+// 16 bytes value by value) the same took 177 and 731.  Read-only loads leave the forward 64 registers in place of 80 and
+// took 104 us, but are not for inputs that the kernel before still writes (heads_wait).
 #pragma once
 #include <math.h>
 

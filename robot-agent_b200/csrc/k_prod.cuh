@@ -38,11 +38,12 @@
 // shared memory and reads 48 KB out of it for 512 cycles of MMAs, 192 bytes a cycle where an SM has 128;
 // in a pair it is 32 + 32 KB (microscaled rows, 128 x 192: 40 + 40 KB for 384 cycles, in a pair 28 + 28).
 //
-// Measured (device time in a graph; 65536 x 1152 rows in 32 groups, n = k = 1152, bf16): y 133 us, dx 131, dw 140, 1.24 to 1.33
-// PFLOP/s, the tensor pipe at 82% of the launch (a plain library product of the same rows and one matrix: 159 us); e2m1
-// 8192 x 16384 x 1152 with 16-bit results 93 us, e4m3 136; x 8192 511 and 955 us (4.3 and 2.3 PFLOP/s). What bounds it:
-// large tiles, shared memory's bandwidth (above); microscaled rows of few stages, the results' way out through
-// shared memory; few rows, the reading of w (64 maps of 512 x 1152: 12 us for 75 MB).
+// Measured (device time in a graph, one set of inputs; 65536 x 1152 rows in 32 groups, n = k = 1152, bf16): y 135 us, dx 136,
+// dw 142, 1.2 to 1.3 PFLOP/s, the tensor pipe at 75 to 82% of the launch (a plain library product of the same rows and one
+// matrix: 159 us); e2m1 8192 x 16384 x 1152 with 16-bit results 95 us, e4m3 139; x 8192 521 and 960 us (4.2 and 2.3
+// PFLOP/s). What bounds it: large tiles, shared memory's bandwidth (above); microscaled rows of few stages, the
+// results' way out through shared memory; few rows, the reading of w (64 maps of 512 x 1152, 75 MB: 16 us from memory,
+// 12 where L2 holds them).
 //
 // Every wait is bounded: by AG_WAIT_NS where the other side owes a stage or an accumulator, by PR_LONG_NS where it
 // may rightly take a whole tile; the latter also ends when a role has given up, in either CTA of a pair

@@ -168,9 +168,11 @@ int smg_group_product(const void* x, int64_t ldx, const void* w, int64_t ldw, in
   const ProdArgs g = prod_fill(off, n_groups, rows, n, k, y, ldy, 0, y_type, err);
   const Operands o = {x, w, ldx, ldw, w_stride, k, k};
   const cudaStream_t st = (cudaStream_t)stream;
-  // Up to 8 rows a group, and weights that do not make it a matter of bandwidth: on 1 to 8 rows of one group
-  // (n = k = 1152) 2.6 us against 6.8, on 24 groups of 512 x 1152 (28 MB) 7.2 against 7.5, on 42 (50 MB) 11.3
-  // against 11.7; on 64 groups (75 MB) 15.2 against 12.3, and on 64 of 1152 x 1152 42 against 31.
+  // Up to 8 rows a group in the mean, and weights that do not make it a matter of bandwidth.  Both sides measured with
+  // the weights in L2 (one set, replayed): on 1 to 8 rows of one group (n = k = 1152) 2.6 us against 6.8, on 24
+  // groups of 512 x 1152 (28 MB) 7.2 against 7.5, on 42 (50 MB) 11.3 against 11.7; on 64 groups (75 MB) 15.2 against
+  // 12.3, and on 64 of 1152 x 1152 42 against 31.  From memory (sets in turn) this side takes 9.1 us on 24 groups and
+  // 14.5 on 42, the other 15.7 on 64: where the two meet then was not measured.
   if ((int64_t)rows <= FEW_ROWS * (int64_t)n_groups && (int64_t)n_groups * n * k <= 24ll << 20) {
     const FewArgs a = {off, n_groups, rows, n, k, x, w, ldx, ldw, w_stride, y, ldy, y_type, err};
     const dim3 grid((n + FEW_W - 1) / FEW_W, n_groups);

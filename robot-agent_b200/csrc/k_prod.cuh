@@ -38,9 +38,9 @@
 // shared memory and reads 48 KB out of it for 512 cycles of MMAs, 192 bytes a cycle where an SM has 128;
 // in a pair it is 32 + 32 KB (microscaled rows, 128 x 192: 40 + 40 KB for 384 cycles, in a pair 28 + 28).
 //
-// Measured (device time in a graph, one set of inputs; 65536 x 1152 rows in 32 groups, n = k = 1152, bf16): y 135 us, dx 136,
+// Measured (device time in a graph, one set of inputs; 65536 x 1152 rows in 32 groups, n = k = 1152, bf16): y 137 us, dx 137,
 // dw 142, 1.2 to 1.3 PFLOP/s, the tensor pipe at 75 to 82% of the launch (a plain library product of the same rows and one
-// matrix: 159 us); e2m1 8192 x 16384 x 1152 with 16-bit results 95 us, e4m3 139; x 8192 521 and 960 us (4.2 and 2.3
+// matrix: 159 us); e2m1 8192 x 16384 x 1152 with 16-bit results 97 us, e4m3 144; x 8192 521 and 960 us (4.2 and 2.3
 // PFLOP/s). What bounds it: large tiles, shared memory's bandwidth (above); microscaled rows of few stages, the
 // results' way out through shared memory; few rows, the reading of w (64 maps of 512 x 1152, 75 MB: 16 us from memory,
 // 12 where L2 holds them).
@@ -176,28 +176,21 @@ DEV uint32_t pr_rank() {
   return r;
 }
 
-// Arrival on the leader's barrier that lies where b does here.  Where it reports data of asynchronous copies that
-// have landed, or a read that is over, it goes without cluster-wide release and acquire: with them on every
-// stage the products ran at 0.4 of this speed.  RELEASE: ordinary writes to this CTA's shared memory come before it
-// (scales, the zeros of dw's last block), and the leader waits with wait_pair.  The fences of both are restricted to
-// shared memory: a full release also waits for the results that the CTA is storing (8192 x 16384 x 1152 in 4 bits
-// 131 us against 96).
-template <bool RELEASE = false>
+// Arrival on the leader's barrier that lies where b does here, and what the leader does once it has seen it (ag_wait<true>
+// or pr_test<true>): release and acquire at cluster scope, since what it reports is this CTA's shared memory (landed
+// copies, scales, the zeros of dw's last block) for instructions that the leader issues.  The fences are
+// restricted to shared memory (arrivals with CTA scope, which PTX does not promise to be enough, took 1 to 4% less:
+// 8192 x 16384 x 1152 in 4 bits 95 us against 97, in 8 bits 139 against 144); full ones also wait for the results that
+// the CTA is storing (on every stage the products ran at 0.4 of their speed, on the scales alone 131 us).
 DEV void pr_arrive_leader(uint64_t* b) {
-  if constexpr (RELEASE)
-    asm volatile(
-        "{\n\t.reg .b32 a;\n\t"
-        "fence.release.sync_restrict::shared::cta.cluster;\n\t"
-        "mapa.shared::cluster.u32 a, %0, 0;\n\t"
-        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(ag_smem(b))
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .b32 a;\n\t"
-        "mapa.shared::cluster.u32 a, %0, 0;\n\t"
-        "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(ag_smem(b))
-        : "memory");
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "fence.release.sync_restrict::shared::cta.cluster;\n\t"
+      "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(ag_smem(b))
+      : "memory");
 }
+DEV void pr_acquire_pair() { asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory"); }
 
 // arrives on b here (PAIR: there and here) when the MMAs issued so far are done
 template <bool PAIR>
@@ -220,15 +213,25 @@ DEV void pr_cluster_sync() {
 }
 
 // whether the phase is over, without waiting
+template <bool CLUSTER>
 DEV bool pr_test(uint64_t* b, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(ag_smem(b)), "r"(parity)
-      : "memory");
+  if constexpr (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(ag_smem(b)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(ag_smem(b)), "r"(parity)
+        : "memory");
   return ok != 0;
 }
 
@@ -448,10 +451,10 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
     return PAIR && (FORM == FORM_Y ? g.n : g.k) - (FORM == FORM_DW ? c.f / g.p_tiles : c.f) * BN <= BN / 2;
   };
   const auto wait = [](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, ag_wait(b, parity)) != 0; };
-  // for ordinary writes of either CTA of a pair, released by pr_arrive_leader<true>
+  // for arrivals from either CTA of a pair
   const auto wait_pair = [](uint64_t* b, uint32_t parity) {
     const bool over = __all_sync(0xffffffffu, ag_wait<PAIR>(b, parity)) != 0;
-    if (PAIR) asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+    if (PAIR) pr_acquire_pair();
     return over;
   };
   if (warp == 0) {   // loads
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
       const ProdTile c = prod_tile<FORM, BN, PAIR>(T, t).uniform();
       const int len = FORM == FORM_DW ? c.r1 - c.r0 : red, nk = (len + BK - 1) / BK;
       const uint32_t acc = j & 1u;
-      if (j >= 2 && !wait(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
+      if (j >= 2 && !wait_pair(&tempty[acc], ((j >> 1) & 1u) ^ 1u)) { ok = false; break; }
       ag_fence_after();
       const uint32_t d = tmem + acc * BN;
       const uint32_t idesc = slim(c) ? (g.idesc & ~(0x3fu << 17)) | (uint32_t)(BN / 16) << 17 : g.idesc;
@@ -507,10 +510,13 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
         const uint32_t ph = (it / STAGES) & 1u;
         const int left = len - kb * BK;
         uint64_t* landed = RELAY ? fixed : full;
-        const bool zeros = PAIR && FORM == FORM_DW && left < BK;   // the other CTA has written zeros into its part
-        if (zeros ? !wait_pair(&landed[s], ph) : !__all_sync(0xffffffffu, ready) && !wait(&landed[s], ph)) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, ready)) {
+          if (!(RELAY ? wait_pair(&landed[s], ph) : wait(&landed[s], ph))) { ok = false; break; }
+        } else if (PAIR) {
+          pr_acquire_pair();   // the arrivals that pr_test saw
+        }
         if (KIND != 16 && kb % S::CHUNK_STAGES == 0 && !wait(&cready[ci & 1u], (ci >> 1) & 1u)) { ok = false; break; }
-        ready = pr_test(&landed[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u);   // the next stage, while this one's MMAs go out
+        ready = pr_test<PAIR>(&landed[(it + 1) % STAGES], ((it + 1) / STAGES) & 1u);   // the next stage, while this one's MMAs go out
         ag_fence_after();
         const unsigned char *p = sP + s * S::P_BYTES, *q = sQ + s * S::Q_BYTES;
         const uint64_t dp = P_MN ? pr_desc_mn(p) : ag_desc(p), dq = Q_MN ? pr_desc_mn(q) : ag_desc(q);
@@ -552,7 +558,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
         if (!wait(&cfull[s], ph)) { ok = false; break; }
         pr_proxy_fence();   // they were written by ordinary copies
         if (PAIR && rank == 1) {
-          if (one) pr_arrive_leader<true>(&cpeer[s]);
+          if (one) pr_arrive_leader(&cpeer[s]);
           continue;
         }
         if (PAIR && !wait_pair(&cpeer[s], ph)) { ok = false; break; }
@@ -629,8 +635,7 @@ __global__ void __launch_bounds__(PR_THREADS(KIND, PAIR), 1)
         }
         __syncwarp();
         if (lane == 0) {
-          if (PAIR && FORM == FORM_DW && tail < BK) pr_arrive_leader<true>(&fixed[s]);
-          else if (PAIR) pr_arrive_leader(&fixed[s]);
+          if (PAIR) pr_arrive_leader(&fixed[s]);
           else pr_arrive(&fixed[s]);
         }
       }

@@ -41,19 +41,20 @@ def test_failure_reaches_both_ctas_of_a_pair():
     assert "while (!ag_wait" not in s                         # no wait without a limit of its own
 
 
-def test_ordinary_writes_cross_a_pair_with_release_and_acquire():
-    """The scales (written by ordinary copies) and the zeros of dw's last block are read by the leader's instructions in the
-    other CTA: they are released and acquired at cluster scope."""
+def test_arrivals_cross_a_pair_with_release_and_acquire():
+    """What one CTA of a pair reports to the other's barriers (landed stages, scales, zeros, read accumulators) is released
+    and acquired at cluster scope, wherever the leader waits for it."""
     s, tc = _code("k_prod.cuh"), _code("tc_util.cuh")
+    assert s.count("mbarrier.arrive.relaxed.cluster.shared::cluster") == 1
     arrive = s[s.index("DEV void pr_arrive_leader"):]
     assert re.search(r"fence\.release\.sync_restrict::shared::cta\.cluster;.*mapa.*mbarrier\.arrive\.relaxed\.cluster", arrive, re.S)
-    assert "mbarrier.try_wait.parity.relaxed.cluster" in tc
-    assert re.search(r"ag_wait<PAIR>.*fence\.acquire\.sync_restrict::shared::cluster\.cluster", s, re.S)
-    assert re.findall(r"pr_arrive_leader(<true>)?\(&cpeer", s) == ["<true>"]
-    assert re.search(r"wait_pair\(&cpeer\[s\]", s)
-    relay = s[s.index("RELAY && warp"):]
-    relay = relay[relay.index("make_uint4(0, 0, 0, 0)"):]
-    assert re.search(r"tail < BK\)\s*pr_arrive_leader<true>\(&fixed", relay) and re.search(r"zeros \? !wait_pair\(&landed", s)
+    assert not re.search(r"mbarrier\.arrive\.shared::cluster", s)               # no arrival there without the fence
+    assert "mbarrier.try_wait.parity.relaxed.cluster" in tc and "mbarrier.test_wait.parity.relaxed.cluster" in s
+    assert re.search(r"ag_wait<PAIR>.*pr_acquire_pair", s, re.S) and "fence.acquire.sync_restrict::shared::cluster.cluster" in s
+    barriers = set(re.findall(r"pr_arrive_leader\(&(\w+)\[", s))
+    assert barriers == {"cpeer", "fixed", "tempty"}
+    assert re.search(r"wait_pair\(&cpeer\[", s) and re.search(r"wait_pair\(&tempty\[", s) and re.search(r"RELAY \? wait_pair\(&landed\[", s)
+    assert re.search(r"pr_test<PAIR>\(&landed", s) and re.search(r"else if \(PAIR\) \{\s*pr_acquire_pair\(\)", s)
 
 
 @pytest.mark.parametrize("name", ["k_mx.cuh", "k_norm.cuh", "k_few.cuh", "k_prod.cuh"])

@@ -7,6 +7,8 @@ memory bank and the scores in 8 or 4 bits.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import products as P
@@ -46,13 +48,18 @@ class MapHeads:
         rows = max(1, z.shape[0])
         loss = 0.5 * e.square().sum() / rows
         # The gradient for the values is e * scale / rows.  Its factor stays out of the 16-bit steps: a mean over many
-        # rows would put f16's values below its smallest ones (65536 rows x 1152: 9 of 10 were lost).
-        _, dw, dgain = self.backward(e.to(z.dtype), f, z, off)
+        # rows would put f16's values below its smallest ones (65536 rows x 1152: 9 of 10 were lost).  In f16 a power of
+        # two goes in where eps is so small that dh, up to |e| / sqrt(eps) in a row of zeros, would not fit.
+        down = 1.0
+        if z.dtype == torch.float16 and self.eps > 0:
+            down = 2.0 ** min(0, 14 + math.floor(math.log2(self.eps) / 2))
+        _, dw, dgain = self.backward((e * down if down != 1 else e).to(z.dtype), f, z, off)
+        step = lr * scale / rows / down
         bad = P.failed(z.device)
         dw.masked_fill_(bad, 0)
         dgain.masked_fill_(bad, 0)
-        self.master.sub_(dw, alpha=lr * scale / rows)
-        self.gain.sub_(dgain, alpha=lr * scale / rows)
+        self.master.sub_(dw, alpha=step)
+        self.gain.sub_(dgain, alpha=step)
         self.w.copy_(self.master)
         return loss.masked_fill_(bad[0], float("nan"))
 

@@ -1,4 +1,6 @@
 """MapHeads.train_step on the B200 against 64 bits: what a step changes, for many rows (where a mean's 1 / rows is small)."""
+import math
+
 import pytest
 
 from conftest import has_gpu
@@ -16,12 +18,11 @@ def unit(v):
     return v / v.norm(dim=-1, keepdim=True)
 
 
-@pytest.mark.parametrize("t", ["f16", "bf16"])
-@pytest.mark.parametrize("counts,dim", [([30000, 0, 35536], 1152), ([4000, 99], 1152), ([5], 64)])
-def test_step_matches_64_bits(t, counts, dim):
-    """The changes of the weights and of the gain, which start at 0 and 1.  With e the error of a value, the gradient for it is
-    e / (sqrt(dim) rows).  Bounds, term by term: e is a difference of 32-bit values; the gradient and dh are each rounded
-    once to the 16-bit type (relative u; below its normal range by half the least spacing); the sums run in 32 bits."""
+def check_step(t, counts, dim, eps=1e-6, zeros=0):
+    """The changes of the weights and of the gain, which start at 0 and 1, with `zeros` rows of zeros.  With e the error of a
+    value, the gradient for it is e / (sqrt(dim) rows).  Bounds, term by term: e is a difference of 32-bit values; the
+    gradient and dh are each rounded once to the 16-bit type (relative u; below its normal range by half the least
+    spacing, of what f16 is scaled by so that 1 / sqrt(eps) fits); the sums run in 32 bits."""
     import torch
     import products_ref as R
     from scenemap_b200 import products as P
@@ -31,12 +32,14 @@ def test_step_matches_64_bits(t, counts, dim):
     P.clear_error()
     rows, off, lr = sum(counts), R.offsets(counts, "cuda"), 1000.0
     z = unit(torch.randn(rows, dim, device="cuda")).to(t)
+    z[:zeros] = 0
     target = unit(torch.randn(rows, dim, device="cuda"))
-    H = MapHeads(len(counts), dim, dtype=t)
+    H = MapHeads(len(counts), dim, dtype=t, eps=eps)
     v = H.forward(z, off, 8, True).values.double()
     loss = H.train_step(z, target, off, lr)
 
-    scale, u, tiny = dim ** -0.5, R.U[t], R.TINY[t] / 2
+    down = 2.0 ** min(0, 14 + math.floor(math.log2(eps) / 2)) if t == torch.float16 else 1.0
+    scale, u, tiny = dim ** -0.5, R.U[t], R.TINY[t] / 2 / down
     e = v * scale - target.double()
     h = z.double()                                       # W = 0
     rstd = 1 / torch.sqrt((h * h).mean(1, keepdim=True) + H.eps)
@@ -58,6 +61,19 @@ def test_step_matches_64_bits(t, counts, dim):
     want = 0.5 * (e * e).sum() / rows
     assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
     assert P.error() == 0
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("counts,dim", [([30000, 0, 35536], 1152), ([4000, 99], 1152), ([5], 64)])
+def test_step_matches_64_bits(t, counts, dim):
+    check_step(t, counts, dim)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("eps", [1e-6, 1e-9, 1e-12, 1e-14])
+def test_step_with_rows_of_zeros(t, eps):
+    """An empty crop's embedding: 1 / rms is 1 / sqrt(eps), and the gradient for its sum that many times its error."""
+    check_step(t, [150, 151], 64, eps, 3)
 
 
 def test_step_with_bad_offsets_changes_nothing():

@@ -38,6 +38,7 @@ class MapHeads:
         dz = P.grouped_dx(dh, self.w, off) + dh        # through W, and past it
         return dz, dw, dgain
 
+    @torch.no_grad()
     def train_step(self, z: torch.Tensor, target: torch.Tensor, off: torch.Tensor, lr: float) -> torch.Tensor:
         """One step of gradient descent on the mean over the rows of |y / sqrt(dim) - target|^2 / 2, target the unit vector of
         the object that row r shows.  Returns the loss (a tensor: nothing waits for it).  A step that finds the device's

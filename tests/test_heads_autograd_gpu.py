@@ -67,3 +67,14 @@ def test_inputs_changed_before_the_gradient(which):
     with torch.inference_mode():                         # inference tensors count no changes
         g = P.norm_add(x.clone(), None, gain)
         P.norm_add_backward(dy, g, gain)
+
+
+def test_training_step_on_tensors_that_require_gradients():
+    """A training step takes its own gradients: tensors of a caller's graph go in as they are, and none of it is recorded."""
+    from scenemap_b200.heads import MapHeads
+    off = R.offsets([20, 12], "cuda")
+    z, target = rnd(32, 64), torch.nn.functional.normalize(torch.randn(32, 64, device="cuda"), dim=1)
+    a, b = MapHeads(2, 64), MapHeads(2, 64)
+    plain = a.train_step(z, target, off, 5.0)
+    loss = b.train_step(z.clone().requires_grad_(), target.clone().requires_grad_(), off, 5.0)
+    assert torch.equal(loss, plain) and not loss.requires_grad and torch.equal(a.master, b.master) and torch.equal(a.gain, b.gain)
